@@ -80,6 +80,23 @@ at::Tensor p2p_moe_combine(const at::Tensor& y_ptrs, int64_t y_byte_offset, cons
                            const c10::optional<at::Tensor>& scores, int64_t hidden, int64_t experts_per_rank, int64_t capacity);
 at::Tensor p2p_moe_pair_dot(const at::Tensor& y_ptrs, int64_t y_byte_offset, const at::Tensor& experts, const at::Tensor& dest_row,
                             const at::Tensor& dout, int64_t experts_per_rank, int64_t capacity);
+at::Tensor paged_kv_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
+                           const at::Tensor& sin, at::Tensor k_pages, at::Tensor v_pages, const at::Tensor& table,
+                           const at::Tensor& starts, const c10::optional<at::Tensor>& counts,
+                           const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale);
+at::Tensor paged_latent_append(const at::Tensor& q_pe, const at::Tensor& kv_a, const at::Tensor& weight, double eps,
+                               const at::Tensor& cos, const at::Tensor& sin, at::Tensor pages, const at::Tensor& table,
+                               const at::Tensor& starts, const c10::optional<at::Tensor>& counts,
+                               const c10::optional<at::Tensor>& scale);
+at::Tensor paged_read(const at::Tensor& pages, const at::Tensor& table, const at::Tensor& lengths, int64_t max_length,
+                      const c10::optional<at::Tensor>& scale, at::ScalarType dtype);
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                           const at::Tensor& starts, const c10::optional<at::Tensor>& counts,
+                           const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale, double scale,
+                           int64_t window);
+at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& q_pe, const at::Tensor& pages, const at::Tensor& table,
+                                  const at::Tensor& starts, const c10::optional<at::Tensor>& counts,
+                                  const c10::optional<at::Tensor>& page_scale, double scale);
 }  // namespace atb
 
 TORCH_LIBRARY(atb200, m) {
@@ -142,4 +159,15 @@ TORCH_LIBRARY(atb200, m) {
     m.def("moe_scatter_bwd(Tensor dout, Tensor slots) -> Tensor", &atb::moe_scatter_bwd);
     m.def("moe_gather_fwd(Tensor y, Tensor slots, Tensor scores) -> Tensor", &atb::moe_gather_fwd);
     m.def("moe_gather_bwd(Tensor dout, Tensor y, Tensor slots, Tensor scores) -> (Tensor, Tensor)", &atb::moe_gather_bwd);
+    m.def("paged_kv_append(Tensor q, Tensor k, Tensor v, Tensor cos, Tensor sin, Tensor(a!) k_pages, Tensor(b!) v_pages, "
+          "Tensor page_table, Tensor starts, Tensor? counts, Tensor(c!)? k_scale, Tensor(d!)? v_scale) -> Tensor",
+          &atb::paged_kv_append);
+    m.def("paged_latent_append(Tensor q_pe, Tensor kv_a, Tensor norm_weight, float eps, Tensor cos, Tensor sin, Tensor(a!) pages, "
+          "Tensor page_table, Tensor starts, Tensor? counts, Tensor(b!)? page_scale) -> Tensor", &atb::paged_latent_append);
+    m.def("paged_read(Tensor pages, Tensor page_table, Tensor lengths, int max_length, Tensor? page_scale, ScalarType dtype) -> Tensor",
+          &atb::paged_read);
+    m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor starts, Tensor? counts, "
+          "Tensor? k_scale, Tensor? v_scale, float scale, int window) -> Tensor", &atb::paged_attention);
+    m.def("paged_latent_attention(Tensor q_latent, Tensor q_pe, Tensor pages, Tensor page_table, Tensor starts, Tensor? counts, "
+          "Tensor? page_scale, float scale) -> Tensor", &atb::paged_latent_attention);
 }

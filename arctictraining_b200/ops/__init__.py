@@ -19,9 +19,15 @@ from .functional import rope_qkv
 from .functional import set_gemm_backend
 from .functional import sumsq
 from .functional import swiglu_interleaved
+from .paged import paged_attention
+from .paged import paged_kv_append
+from .paged import paged_kv_read
+from .paged import paged_latent_append
+from .paged import paged_latent_attention
 
 __all__ = [
     "reference", "IGNORE_INDEX", "LAUNCH_COUNTER", "COMM_COUNTER", "accumulate_lp_grad", "adamw_step", "attention",
-    "fused_linear_cross_entropy", "fused_linear_logprobs", "gemm", "linear", "linear_swiglu", "mlp_swiglu", "rms_norm", "rope", "rope_attention", "rope_qkv", "set_gemm_backend",
+    "fused_linear_cross_entropy", "fused_linear_logprobs", "gemm", "linear", "linear_swiglu", "mlp_swiglu", "paged_attention", "paged_kv_append",
+    "paged_kv_read", "paged_latent_append", "paged_latent_attention", "rms_norm", "rope", "rope_attention", "rope_qkv", "set_gemm_backend",
     "sumsq", "swiglu_interleaved",
 ]

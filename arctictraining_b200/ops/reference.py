@@ -205,3 +205,126 @@ def topk_gating(logits: torch.Tensor, top_k: int, normalize: bool) -> Tuple[torc
     if normalize:
         scores = scores / scores.sum(-1, keepdim=True)
     return probs, scores, order
+
+
+# ------------------------------------------------------------------------------------------------ paged generation cache
+E4M3_MAX = 448.0
+E4M3_TINY = 2.0**-100
+
+
+def quantize_rows_e4m3(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of ``x [..., D]`` as e4m3 values and one fp32 scale each: largest magnitude / 448 (at least 2^-100 / 448, so
+    that a row of zeros has one too)."""
+    xf = x.float()
+    scale = xf.abs().amax(-1).clamp(min=E4M3_TINY) / E4M3_MAX
+    return (xf * (1.0 / scale).unsqueeze(-1)).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn), scale
+
+
+def _paged_slots(page_table, starts, counts, S: int, pages: torch.Tensor):
+    """(written, page id, offset), each ``[B, S]``, of the new tokens' places."""
+    P, page = pages.shape[0], pages.shape[2]
+    B, W = page_table.shape
+    j = torch.arange(S, device=pages.device).view(1, S)
+    pos = starts.long().view(B, 1) + j
+    ok = (starts.view(B, 1) >= 0) & (pos < W * page)
+    if counts is not None:
+        ok = ok & (j < counts.view(B, 1))
+    if W == 0:
+        return ok, pos, pos
+    pid = torch.gather(page_table.long(), 1, (pos // page).clamp(0, W - 1))
+    return ok & (pid >= 0) & (pid < P), pid, pos % page
+
+
+def _paged_write(pages, scales, rows, page_table, starts, counts) -> None:
+    ok, pid, off = _paged_slots(page_table, starts, counts, rows.shape[1], pages)
+    pid, off, rows = pid[ok], off[ok], rows[ok]
+    if scales is None:
+        pages[pid, :, off] = rows.to(pages.dtype)
+    else:
+        values, sc = quantize_rows_e4m3(rows)
+        pages.view(torch.uint8)[pid, :, off] = values.view(torch.uint8)
+        scales[pid, :, off] = sc
+
+
+def _paged_gather(pages, scales, page_table) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The cached rows in fp32 ``[B, H, W * page, D]`` and which of them lie on a page that exists ``[B, W * page]``."""
+    P, H, page, D = pages.shape
+    B, W = page_table.shape
+    if P == 0 or W == 0:
+        return (torch.zeros(B, H, W * page, D, device=pages.device),
+                torch.zeros(B, W * page, device=pages.device, dtype=torch.bool))
+    ids = page_table.long()
+    held = (ids >= 0) & (ids < P)
+    ids = ids.clamp(0, P - 1)
+    if scales is None:
+        x = pages[ids].float()
+    else:
+        x = pages.view(torch.uint8)[ids].view(torch.float8_e4m3fn).float() * scales[ids].unsqueeze(-1)
+    return x.permute(0, 2, 1, 3, 4).reshape(B, H, W * page, D), held.repeat_interleave(page, dim=1)
+
+
+def paged_kv_append(q, k, v, cos, sin, k_pages, v_pages, page_table, starts, counts=None, k_scale=None, v_scale=None):
+    d2 = q.shape[-1] // 2
+    c, s = cos.unsqueeze(2), sin.unsqueeze(2)
+
+    def turn(x):
+        x1, x2 = x[..., :d2].float(), x[..., d2:].float()
+        return torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), dim=-1)
+
+    _paged_write(k_pages, k_scale, turn(k), page_table, starts, counts)
+    _paged_write(v_pages, v_scale, v.float(), page_table, starts, counts)
+    return turn(q).to(q.dtype)
+
+
+def paged_latent_append(q_pe, kv_a, norm_weight, eps, cos, sin, pages, page_table, starts, counts=None, page_scale=None):
+    R = norm_weight.shape[0]
+    latent = kv_a[..., :R].float()
+    latent = latent * torch.rsqrt(latent.pow(2).mean(-1, keepdim=True) + eps) * norm_weight.float()
+    k_pe = rope_apply(kv_a[..., R:].float().unsqueeze(2), cos, sin)
+    _paged_write(pages, page_scale, torch.cat((latent.unsqueeze(2), k_pe), dim=-1), page_table, starts, counts)
+    return rope_apply(q_pe, cos, sin)
+
+
+def paged_read(pages, page_table, lengths, max_length: int, page_scale, dtype) -> torch.Tensor:
+    x, held = _paged_gather(pages, page_scale, page_table)
+    B, H, L, D = x.shape
+    n = min(max_length, L)
+    held = held[:, :n] & (torch.arange(n, device=pages.device).view(1, n) < lengths.view(B, 1))
+    out = torch.zeros(B, max_length, H, D, device=pages.device, dtype=dtype)
+    out[:, :n] = torch.where(held.view(B, n, 1, 1), x[:, :, :n].transpose(1, 2), torch.zeros((), device=pages.device)).to(dtype)
+    return out
+
+
+def _paged_softmax_product(q, k, v, held, starts, counts, scale: float, window) -> torch.Tensor:
+    """``q [B, S, Hq, D]`` against fp32 ``k / v [B, Hkv, L, .]``; a query that sees nothing gets zeros."""
+    B, S, Hq, _ = q.shape
+    Hkv, L = k.shape[1:3]
+    if L == 0 or q.numel() == 0:
+        return torch.zeros(B, S, Hq, v.shape[-1], device=q.device, dtype=q.dtype)
+    at = torch.arange(L, device=q.device).view(1, 1, L)
+    j = torch.arange(S, device=q.device).view(1, S, 1)
+    mine = starts.long().view(B, 1, 1) + j
+    seen = (at <= mine) & held.view(B, 1, L)
+    if window:
+        seen = seen & (at > mine - window)
+    if counts is not None:
+        seen = seen & (j < counts.view(B, 1, 1))
+    any_query = seen.any(1).view(B, 1, L, 1)  # values that no query sees may be anything, NaN too
+    v = torch.where(any_query, v, torch.zeros((), device=v.device, dtype=v.dtype))
+    qf = q.float().view(B, S, Hkv, Hq // Hkv, -1).permute(0, 2, 3, 1, 4)
+    scores = torch.matmul(qf, k.unsqueeze(2).transpose(-1, -2)) * scale
+    scores = scores.masked_fill(~seen.view(B, 1, 1, S, L), float("-inf"))
+    p = torch.softmax(scores, dim=-1).masked_fill(~seen.any(-1).view(B, 1, 1, S, 1), 0.0)
+    return torch.matmul(p, v.unsqueeze(2)).permute(0, 3, 1, 2, 4).reshape(B, S, Hq, -1).to(q.dtype)
+
+
+def paged_attention(q, k_pages, v_pages, page_table, starts, counts, k_scale, v_scale, scale: float, window) -> torch.Tensor:
+    k, held = _paged_gather(k_pages, k_scale, page_table)
+    v, _ = _paged_gather(v_pages, v_scale, page_table)
+    return _paged_softmax_product(q, k, v, held, starts, counts, scale, window)
+
+
+def paged_latent_attention(q_latent, q_pe, pages, page_table, starts, counts, page_scale, scale: float) -> torch.Tensor:
+    k, held = _paged_gather(pages, page_scale, page_table)
+    return _paged_softmax_product(torch.cat((q_latent, q_pe), dim=-1), k, k[..., : q_latent.shape[-1]], held, starts, counts,
+                                  scale, None)
