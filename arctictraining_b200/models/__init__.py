@@ -6,5 +6,7 @@ from .causal_lm import CausalLMOutput
 from .factory import HFModelFactory
 from .factory import LigerModelFactory
 from .factory import ModelFactory
+from .kv_cache import PagedKVCache
 
-__all__ = ["ArchConfig", "load_arch_config", "CausalLM", "CausalLMOutput", "HFModelFactory", "LigerModelFactory", "ModelFactory"]
+__all__ = ["ArchConfig", "load_arch_config", "CausalLM", "CausalLMOutput", "HFModelFactory", "LigerModelFactory", "ModelFactory",
+           "PagedKVCache"]

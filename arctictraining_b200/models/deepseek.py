@@ -72,10 +72,14 @@ class MLAQuery(nn.Module):
         else:
             self.q_proj = Linear(hidden, self.heads * (self.nope + self.rope), dtype=dtype, device=device)
 
-    def forward(self, x: torch.Tensor, ctx: ForwardContext) -> torch.Tensor:
+    def project(self, x: torch.Tensor) -> torch.Tensor:
+        """The queries before rotation."""
         B, S, _ = x.shape
         q = self.q_b_proj(self.q_a_layernorm(self.q_a_proj(x))) if hasattr(self, "q_a_proj") else self.q_proj(x)
-        q = q.view(B, S, self.heads, self.nope + self.rope)
+        return q.view(B, S, self.heads, self.nope + self.rope)
+
+    def forward(self, x: torch.Tensor, ctx: ForwardContext) -> torch.Tensor:
+        q = self.project(x)
         q_pe = ops.rope(q[..., self.nope :].contiguous(), ctx.cos, ctx.sin)
         return torch.cat([q[..., : self.nope], q_pe], dim=-1)
 
@@ -139,8 +143,36 @@ class MLAttention(nn.Module):
             o = ops.attention(q, k, v, ctx.cu_seqlens, ctx.max_seqlen, True, ctx.attn_impl, scale=self.scale)
         return o[..., : self.vd].reshape(B, S, self.heads * self.vd)
 
+    def _forward_paged(self, x: torch.Tensor, ctx: ForwardContext, residual: Optional[torch.Tensor]) -> torch.Tensor:
+        """Generation step over a paged latent cache.  Few new tokens use the absorbed form: the key half of ``kv_b_proj``
+        is applied to the queries, attention runs on the latent rows themselves, the value half turns the weighted latents
+        into heads.  A prompt (or an adapted ``kv_b_proj``) expands the latents that it reads back."""
+        B, S, _ = x.shape
+        cache, kv, H = ctx.kv_cache, self.kv, self.heads
+        q = self.q.project(x)
+        q_nope = q[..., : kv.nope]
+        norm = kv.kv_a_layernorm
+        q_pe = cache.append_latent(self.layer_idx, q[..., kv.nope :], kv.kv_a_proj_with_mqa(x), norm.weight, norm.eps, ctx.cos, ctx.sin)
+        if S <= cache.draft_tokens and type(kv.kv_b_proj) is Linear:
+            w = kv.kv_b_proj.weight.view(H, kv.nope + kv.vd, kv.rank)
+            q_latent = torch.einsum("bshn,hnr->bshr", q_nope, w[:, : kv.nope])
+            latent = cache.attend_latent(self.layer_idx, q_latent, q_pe, self.scale)
+            o = torch.einsum("bshr,hvr->bshv", latent, w[:, kv.nope :])
+        else:
+            rows = cache.read(self.layer_idx, S, x.dtype)[0].squeeze(2)
+            L = rows.shape[1]
+            e = kv.kv_b_proj(rows[..., : kv.rank].contiguous()).view(B, L, H, kv.nope + kv.vd)
+            k = torch.cat([e[..., : kv.nope], rows[..., kv.rank :].unsqueeze(2).expand(B, L, H, kv.rope)], dim=-1)
+            v = F.pad(e[..., kv.nope :], (0, max(0, self.qk - self.vd)))
+            o = cache.prompt_attention(torch.cat([q_nope, q_pe], dim=-1), k, v, self.scale, attn_impl=ctx.attn_impl)[..., : self.vd]
+        return _project_with_residual(self.o_proj, o.reshape(B, S, H * self.vd), residual)
+
     def forward(self, x: torch.Tensor, ctx: ForwardContext, residual: Optional[torch.Tensor] = None,
                 shared_kv=None, query: Optional[MLAQuery] = None) -> torch.Tensor:
+        if ctx.kv_cache is not None and not isinstance(ctx.kv_cache, list):
+            if shared_kv is not None or query is not None:
+                raise NotImplementedError("layers that share another layer's keys and values generate with the dense cache only")
+            return self._forward_paged(x, ctx, residual)
         q = (query or self.q)(x, ctx)
         k, v = shared_kv if shared_kv is not None else self.kv(x, ctx)
         return _project_with_residual(self.o_proj, self.attend(q, k, v, ctx), residual)

@@ -5,7 +5,8 @@ Used where training needs samples from the model itself (the MLP speculator's ge
 generates through Hugging Face's ``DynamicCache`` and also returns the final hidden state of every processed position
 (projects/mlp_speculator/train.py:224-291); this does the same on the native model: the prompt is processed once, every
 further token costs one forward of a single position, and the layers run through their usual (engine-wrapped) forward
-so that ZeRO-3 parameter gathering keeps working.
+so that ZeRO-3 parameter gathering keeps working.  The cache is a pair of growing tensors per layer, or a
+:class:`~arctictraining_b200.models.kv_cache.PagedKVCache` that the caller gives.
 """
 
 from __future__ import annotations
@@ -15,6 +16,8 @@ from typing import Tuple
 
 import torch
 import torch.nn.functional as F
+
+from .kv_cache import PagedKVCache
 
 
 @torch.no_grad()
@@ -26,25 +29,38 @@ def generate(
     temperature: float = 1.0,
     top_k: int = 10,
     generator: Optional[torch.Generator] = None,
+    cache: Optional[PagedKVCache] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Returns ``(tokens [B, S0 + new], hidden [B, S0 + new - 1, H])``: the prompt followed by the generated tokens, and
     the final (normed) hidden state of every position that was fed to the model (the state at position ``t`` predicts
-    token ``t + 1``)."""
+    token ``t + 1``).
+
+    With a paged ``cache`` the prompt continues what the cache holds (``input_ids`` are the tokens behind it), and every token
+    that was fed to the model stays there: all but the last one returned, which starts the next call's prompt."""
     assert input_ids.dim() == 2, "generate: input_ids must be [batch, length]"
     B, S0 = input_ids.shape
     dev = input_ids.device
     n_layers = len(model.model.layers)
-    cache = [None] * n_layers
+    if cache is not None:
+        if cache.batch != B:
+            raise ValueError(f"generate: the cache holds {cache.batch} sequences, the prompt {B}")
+        cache.reserve(S0 + max_new_tokens - 1)
+    kv = cache if cache is not None else [None] * n_layers
     tokens = input_ids
     step_ids, pos0 = input_ids, 0
     hidden_parts = []
     lm_w = model.lm_head.weight
     for _ in range(max_new_tokens):
         S = step_ids.shape[1]
-        position_ids = torch.arange(pos0, pos0 + S, device=dev).unsqueeze(0).expand(B, S)
+        if cache is not None:
+            position_ids = cache.positions(S)
+        else:
+            position_ids = torch.arange(pos0, pos0 + S, device=dev).unsqueeze(0).expand(B, S)
         ctx = model.model.make_context(position_ids, "sdpa")
-        ctx.kv_cache = cache
+        ctx.kv_cache = kv
         h = model.model(step_ids, position_ids, ctx)
+        if cache is not None:
+            cache.advance(S)
         hidden_parts.append(h)
         logits = F.linear(h[:, -1], lm_w).float()
         if do_sample:

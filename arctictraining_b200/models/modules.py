@@ -36,8 +36,9 @@ class ForwardContext:
     extras: Dict[str, Any] = field(default_factory=dict)
     # rotary tables for arbitrary positions (used for the whole sequence when rotation happens after the Ulysses exchange)
     rope_fn: Optional[Any] = None
-    # generation: one (keys, values) pair per layer, [B, S_past, Hkv, D], grown by every call (None: training / scoring)
-    kv_cache: Optional[list] = None
+    # generation: a PagedKVCache, or one (keys, values) pair per layer, [B, S_past, Hkv, D], grown by every call (None:
+    # training / scoring)
+    kv_cache: Optional[Any] = None
 
 
 class RMSNorm(nn.Module):
@@ -95,6 +96,17 @@ class Attention(nn.Module):
             self.q_norm = RMSNorm(self.d, cfg["rms_norm_eps"], dtype=dtype, device=device)
             self.k_norm = RMSNorm(self.d, cfg["rms_norm_eps"], dtype=dtype, device=device)
 
+    def _forward_paged(self, x: torch.Tensor, ctx: ForwardContext, residual: Optional[torch.Tensor]) -> torch.Tensor:
+        """Generation step over a paged cache: rotation and cache write in one operator, attention over the pages."""
+        B, S, _ = x.shape
+        q, k, v = self.qkv_proj(x).split([self.hq * self.d, self.hkv * self.d, self.hkv * self.d], dim=-1)
+        q, k, v = (t.view(B, S, -1, self.d) for t in (q, k, v))
+        if self.qk_norm:
+            q, k = self.q_norm(q.contiguous()), self.k_norm(k.contiguous())
+        q = ctx.kv_cache.append(self.layer_idx, q, k, v, ctx.cos, ctx.sin)
+        o = ctx.kv_cache.attend(self.layer_idx, q, window=self.window, attn_impl=ctx.attn_impl)
+        return _project_with_residual(self.o_proj, o.reshape(B, S, self.hq * self.d), residual)
+
     def project_qkv(self, x: torch.Tensor, ctx: ForwardContext):
         B, S, _ = x.shape
         qkv = self.qkv_proj(x)
@@ -138,7 +150,8 @@ class Attention(nn.Module):
     def forward(self, x: torch.Tensor, ctx: ForwardContext, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         B, S, _ = x.shape
         if ctx.kv_cache is not None:
-            return self._forward_cached(x, ctx, residual)
+            paged = not isinstance(ctx.kv_cache, list)
+            return self._forward_paged(x, ctx, residual) if paged else self._forward_cached(x, ctx, residual)
         if (
             ctx.sp is not None and hasattr(ctx.sp, "fused_attention_block") and not self.qk_norm
             and type(self.qkv_proj) is Linear and self.qkv_proj.bias is None

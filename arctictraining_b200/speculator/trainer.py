@@ -15,6 +15,7 @@ from __future__ import annotations
 import os
 from typing import Any
 from typing import Dict
+from typing import Literal
 from typing import Union
 
 import torch
@@ -196,6 +197,8 @@ class MLPSpeculatorTrainerConfig(TrainerConfig):
     gen_train_micro_batch_size: int = 32
     gen_prompt_length: int = 64
     gen_seq_length: int = 256
+    gen_kv_cache: Literal["dense", "paged", "paged_e4m3"] = "dense"
+    """ Cache of the generating model: tensors that grow by concatenation, pages of fixed size, or pages of 8-bit rows. """
 
     @model_validator(mode="after")
     def _check_gen_train(self) -> Self:
@@ -248,10 +251,17 @@ class MLPSpeculatorTrainer(ArcticLSTMSpeculatorTrainer):
     def generate(self, prompts: torch.Tensor, new_tokens: int, do_sample: bool = True):
         """Sampled (top-k 10) continuation with a key/value cache; returns ``(tokens, hidden states)``."""
         from ..models.generation import generate
+        from ..models.kv_cache import PagedKVCache
 
+        module, cache = self.model_unwrapped, None
+        if self.config.gen_kv_cache != "dense":
+            cache = PagedKVCache.for_model(
+                module.config, prompts.shape[0], prompts.shape[1] + new_tokens, e4m3=self.config.gen_kv_cache == "paged_e4m3",
+                dtype=module.lm_head.weight.dtype, device=prompts.device,
+            )
         self.model.eval()
         try:
-            return generate(self.model_unwrapped, prompts, new_tokens, do_sample=do_sample)
+            return generate(module, prompts, new_tokens, do_sample=do_sample, cache=cache)
         finally:
             self.model.train()
 
