@@ -4,6 +4,9 @@
 // Query j of a sequence stands at position p = starts + j and sees the cached positions max(0, p - window + 1) .. p:
 // o = sum_t e^(s_t - m) v_t / sum_t e^(s_t - m), s_t = scale q.k_t, in one pass over the keys with the running maximum m.
 // The latent form has one key row [latent | rotary] for all heads and the latent itself as value.
+#include <atomic>
+#include <type_traits>
+
 #include "paged_common.cuh"
 
 namespace atb {
@@ -22,6 +25,717 @@ struct AttnArgs {
     float scale;
 };
 
+// ---- schedule ---------------------------------------------------------------------------------------------------------
+// Work is counted in rounds of `NK` keys of one item (sequence, cache head, tile of query rows).  The rounds of all items
+// stand in one line and every CTA takes an equal piece of it, so a batch of very different lengths loads all SMs alike
+// and a single long sequence is spread over all of them.  A CTA that covers an item alone writes the result; otherwise it
+// leaves (maximum, sum, weighted values) of its piece in the workspace, and the join kernel adds the pieces in their
+// order.  No atomics: the same inputs give the same bits.
+struct Range {  // the cached positions that the queries of one sequence see
+    int start, total, low, first, rounds;  // positions [low, total); counted from `first`, a multiple of NK
+};
+__device__ __forceinline__ Range seq_range(const AttnArgs& a, int b, int NK) {
+    Range r;
+    r.start = a.starts[b];
+    const int count = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
+    const int64_t cap = (int64_t)a.W * a.page, end = (int64_t)r.start + count;
+    r.total = count == 0 ? 0 : (int)max((int64_t)0, min(end, cap));
+    r.low = a.window > 0 ? (int)max((int64_t)0, min((int64_t)r.start + 1 - a.window, (int64_t)r.total)) : 0;
+    r.first = r.low / NK * NK;
+    r.rounds = max(1, (r.total - r.first + NK - 1) / NK);  // a sequence that sees nothing has one round, fully masked
+    return r;
+}
+
+// Sum of the rounds of the sequences before `upto`, and of all: by a CTA of 128 threads.
+__device__ __forceinline__ void sum_rounds(const AttnArgs& a, int B, int NK, int upto, int64_t& before, int64_t& all, int64_t* scratch) {
+    int64_t x = 0, y = 0;
+    for (int b = threadIdx.x; b < B; b += 128) {
+        const int n = seq_range(a, b, NK).rounds;
+        y += n;
+        if (b < upto) x += n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        scratch[threadIdx.x >> 5] = x;
+        scratch[4 + (threadIdx.x >> 5)] = y;
+    }
+    __syncthreads();
+    before = scratch[0] + scratch[1] + scratch[2] + scratch[3];
+    all = scratch[4] + scratch[5] + scratch[6] + scratch[7];
+}
+
+// The sequence that holds round `at` of the line (every sequence has `per` items), and its first round.
+__device__ __forceinline__ void find_round(const AttnArgs& a, int B, int NK, int64_t per, int64_t at, int& b_out, int64_t& first_out,
+                                           int64_t& all, int64_t* scratch) {
+    // thread i looks at sequences [i n, (i + 1) n)
+    const int n = (B + 127) / 128, b0 = threadIdx.x * n, b1 = min(B, b0 + n);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += seq_range(a, b, NK).rounds;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) scratch[warp] = incl;
+    __syncthreads();
+    int64_t base = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < warp) base += scratch[w];
+        all += scratch[w];
+    }
+    all *= per;
+    int64_t lo = (base + incl - mine) * per;
+    // `at` is given as a fraction of the line: CTA c starts at c * all / CTAs
+    const int64_t target = at * all / gridDim.x;
+    if (target >= lo && target < lo + mine * per) {
+        int b = b0;
+        while (true) {
+            const int64_t r = (int64_t)seq_range(a, b, NK).rounds * per;
+            if (target < lo + r) break;
+            lo += r;
+            ++b;
+        }
+        scratch[8] = b;
+        scratch[9] = lo;
+    }
+    __syncthreads();
+    b_out = (int)scratch[8];
+    first_out = scratch[9];
+}
+
+// ---- tensor-core pieces -----------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// c += a b for a 16 x 16, b 16 x 8 of 16-bit elements, fp32 sums
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<bf16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<bf16>(float lo, float hi) {
+    const bf162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<bf16>(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const bf162*>(&u)); }
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool full) {  // asynchronous; zeros where not `full`
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool full) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(full ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// whether some value of the step is an infinity or a NaN (all bits of its exponent set)
+template <typename P, int N, int KP, int CPR, typename F>
+__device__ __forceinline__ bool values_not_finite(F&& load) {
+    constexpr uint32_t e = std::is_same<P, bf16>::value ? 0x7f80u : 0x7c00u;
+    bool bad = false;
+#pragma unroll 1
+    for (int kp = 0; kp < KP; ++kp)
+#pragma unroll
+        for (int k = 0; k < CPR; k += 2) {
+            uint32_t v[N];
+            load(kp, k, v);
+#pragma unroll
+            for (int x = 0; x < N; ++x) bad = bad || (v[x] & e) == e || ((v[x] >> 16) & e) == e;
+        }
+    return __any_sync(0xffffffffu, bad);
+}
+
+// ---- attention over grouped heads --------------------------------------------------------------------------------------
+// Bound by memory: 4 Hq / Hkv flops a cached element.  A CTA of four warps serves the query rows (new token, head of the
+// group) of one cache head, so that a cached row is read once for all of them; rows fill the 16-row side of the matrix
+// instruction.  WR warps stand along the rows (1, 2 or 4 tiles of 16) and 4 / WR rings of warps along the keys: each ring
+// streams its own keys through its own shared-memory stages (cp.async, kStages deep) and keeps its own running maximum,
+// sum and weighted values; with one warp a ring nothing in the loop waits for another warp.  The rings are added at the end
+// of a piece.  Eight-bit rows are turned into fp16 (exactly) on their way into the instruction, the scale of a key
+// multiplies its score, and that of a value goes into the exponent of its probability, with a running maximum of its own,
+// so that probabilities stay within (0, 1] whatever the scales are.
+// Probabilities are rounded to the 16-bit type of the instruction (fp16 for e4m3 values): the same size of error as the
+// final rounding of the result.  Scores, maxima, sums and weighted values are fp32.
+constexpr int kStages = 3;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <bool E4M3, int DP>
+struct Shape {
+    static constexpr int kRowBytes = DP * (E4M3 ? 1 : 2);
+    // keys a warp loads per stage: 8 KB of keys and values where a row allows it
+    static constexpr int kKeys = kRowBytes >= 256 ? 16 : kRowBytes == 128 ? 32 : 64;
+    static constexpr int kRound = 4 * kKeys;  // keys of a round of the CTA
+    // per warp and stage: keys, values, (scales)
+    static constexpr int kStageBytes = 2 * kKeys * kRowBytes + (E4M3 ? 2 * kKeys * 4 : 0);
+    static constexpr int kRingBytes = kStages * 4 * kStageBytes;
+    static constexpr int kOutBytes = 4 * 16 * (DP + 4) * 4;  // the rings' results when they are added
+    static constexpr int kSmem = kRingBytes > kOutBytes ? kRingBytes : kOutBytes;
+};
+
+template <typename T, bool E4M3, int DP, int WR>
+__global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, float* __restrict__ part_ml, float* __restrict__ part_o) {
+    using Sh = Shape<E4M3, DP>;
+    using P = typename std::conditional<E4M3, __half, T>::type;  // type of the matrix instruction
+    constexpr int WK = 4 / WR, KW = Sh::kKeys, TK = KW * WR, NK = Sh::kRound, RB = Sh::kRowBytes;
+    constexpr int CPR = RB / 16;         // 16-byte chunks of a row
+    constexpr int KB = KW < 32 ? KW : 32;  // keys of one softmax step
+    constexpr int kVal = E4M3 ? 8 : 4;     // registers of two 16-byte chunks of 16 values
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int64_t scratch[16];
+    __shared__ uint32_t s_valid[4][kStages][2];
+    __shared__ float s_ml[4][16][2];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int wr = warp % WR, wk = warp / WR;
+    const int g = lane >> 2, c = lane & 3;
+    const int G = a.Hq / a.Hkv, M = a.S * G;
+    const int row_tiles = (M + 16 * WR - 1) / (16 * WR);
+    const int64_t per = (int64_t)a.Hkv * row_tiles;
+
+    int b;
+    int64_t line, all;
+    find_round(a, B, NK, per, blockIdx.x, b, line, all, scratch);
+    int64_t at = (int64_t)blockIdx.x * all / gridDim.x;
+    const int64_t to = ((int64_t)blockIdx.x + 1) * all / gridDim.x;
+    if (at >= to) return;
+    const int64_t began = at;
+    Range rg = seq_range(a, b, NK);
+
+    const uint32_t ring = smem_addr(smem) + wk * WR * kStages * Sh::kStageBytes;
+    // of a stage: keys of all warps of the ring, values, key scales, value scales
+    constexpr int kK = 0, kV = WR * KW * RB, kSK = 2 * WR * KW * RB, kSV = kSK + WR * KW * 4, kStage = WR * Sh::kStageBytes;
+
+    while (at < to) {
+        while (at >= line + rg.rounds * per) {
+            line += rg.rounds * per;
+            ++b;
+            rg = seq_range(a, b, NK);
+        }
+        const int64_t in_seq = at - line;
+        const int item = (int)(in_seq / rg.rounds);  // (cache head, row tile)
+        const int r0 = (int)(in_seq - (int64_t)item * rg.rounds);
+        const int r1 = (int)min((int64_t)rg.rounds, r0 + (to - at));
+        const int h = item / row_tiles, row_base = (item - h * row_tiles) * 16 * WR + wr * 16;
+
+        // query rows of this lane, and the positions that they see
+        int row[2], hi[2], lo[2];
+        uint32_t q[DP / 16][4];
+        float fac[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            row[i] = row_base + g + 8 * i;
+            const int j = min(row[i], M - 1) / G;
+            hi[i] = (int)min((int64_t)rg.start + j, (int64_t)rg.total - 1);
+            lo[i] = a.window > 0 ? (int)max((int64_t)0, (int64_t)rg.start + j + 1 - a.window) : 0;
+            const T* src = (const T*)a.q + b * a.q_b + (int64_t)j * a.q_s + (int64_t)(h * G + min(row[i], M - 1) % G) * a.q_h;
+            const bool real = row[i] < M;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                if (E4M3) {  // elements 4 c .. 4 c + 3 of the chunk, the order in which the keys' bytes arrive
+                    uint2 u = make_uint2(0, 0);
+                    if (real && k * 16 < a.D) u = *reinterpret_cast<const uint2*>(src + k * 16 + 4 * c);
+                    q[k][i] = u.x;
+                    q[k][i + 2] = u.y;
+                } else {
+                    const bool in = real && k * 16 < a.D;
+                    q[k][i] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 2 * c) : 0u;
+                    q[k][i + 2] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8 + 2 * c) : 0u;
+                }
+            }
+            fac[i] = a.scale * kLog2e;
+        }
+        if (E4M3 && std::is_same<T, bf16>::value) {
+            // bf16 queries become fp16 after a power of two per row that brings their largest element to [2^14, 2^15):
+            // exact down to 2^-28 of that element
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float m = 0.f;
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    const float2 x = unpack2<T>(q[k][i]), y = unpack2<T>(q[k][i + 2]);
+                    m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+                }
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const int e = (__float_as_uint(m) >> 23) & 255;
+                const int field = e == 0 || e == 255 ? 127 : min(268 - e, 253);
+                const float up = __uint_as_float((uint32_t)field << 23);
+                fac[i] *= __uint_as_float((uint32_t)(254 - field) << 23);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    const float2 x = unpack2<T>(q[k][i]), y = unpack2<T>(q[k][i + 2]);
+                    q[k][i] = pack2<__half>(x.x * up, x.y * up);
+                    q[k][i + 2] = pack2<__half>(y.x * up, y.y * up);
+                }
+            }
+        }
+        int min_hi = min(hi[0], hi[1]), max_lo = max(lo[0], lo[1]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            min_hi = min(min_hi, __shfl_xor_sync(0xffffffffu, min_hi, o));
+            max_lo = max(max_lo, __shfl_xor_sync(0xffffffffu, max_lo, o));
+        }
+
+        const int key0 = rg.first + wk * TK;  // of the ring's tile in round 0 of the item
+        const int n = r1 - r0;
+        const int64_t head_rows = (int64_t)h * a.page;
+        // page of the key that this lane looks up for tile t (KW keys a warp; lanes beyond them idle; 64 keys: two a lane)
+        constexpr int LK = KW > 32 ? 2 : 1;
+        int pid_next[LK];
+        auto look_up = [&](int t) {
+#pragma unroll
+            for (int x = 0; x < LK; ++x) {
+                const int key = key0 + (r0 + t) * NK + wr * KW + lane + 32 * x;
+                pid_next[x] = -1;
+                if (t < n && (KW >= 32 || lane < KW) && key >= rg.low && key < rg.total) pid_next[x] = a.table[b * a.table_stride + key / a.page];
+            }
+        };
+        auto issue = [&](int t) {  // the copies of tile t of this piece
+            if (t < n) {
+                const int st = t % kStages;
+                const uint32_t base = ring + st * kStage;
+                int64_t off[LK];
+                bool ok[LK];
+#pragma unroll
+                for (int x = 0; x < LK; ++x) {
+                    const int key = key0 + (r0 + t) * NK + wr * KW + lane + 32 * x;
+                    ok[x] = pid_next[x] >= 0 && pid_next[x] < a.P;
+                    const int64_t r = head_rows + key % a.page;
+                    off[x] = ok[x] ? pid_next[x] * a.k_page + r * a.D : 0;
+                    const uint32_t bits = __ballot_sync(0xffffffffu, ok[x]);
+                    if (lane == 0) s_valid[warp][st][x] = bits;
+                    if (E4M3 && (KW >= 32 || lane < KW)) {
+                        const int64_t so = ok[x] ? pid_next[x] * a.ks_page + r : 0;
+                        const uint32_t d = base + kSK + (wr * KW + lane + 32 * x) * 4;
+                        copy4(d, a.k_scale + so, ok[x]);
+                        copy4(d + (kSV - kSK), a.v_scale + so, ok[x]);
+                    }
+                }
+                constexpr int kIter = KW * CPR / 32;
+#pragma unroll
+                for (int i = 0; i < kIter; ++i) {
+                    const int id = i * 32 + lane, key = id / CPR, ch = id % CPR;
+                    const int64_t o = __shfl_sync(0xffffffffu, LK == 2 && i * 32 / CPR >= 32 ? off[LK - 1] : off[0], key & 31);
+                    const bool full = __shfl_sync(0xffffffffu, LK == 2 && i * 32 / CPR >= 32 ? ok[LK - 1] : ok[0], key & 31) &&
+                                      ch * 16 < a.D * (E4M3 ? 1 : 2);
+                    const int64_t byte = full ? (E4M3 ? o : o * 2) + ch * 16 : 0;
+                    const uint32_t d = base + (wr * KW + key) * RB + ((ch ^ (key & 7)) & (CPR - 1)) * 16;
+                    copy16(d + kK, (const uint8_t*)a.k_pages + byte, full);
+                    copy16(d + kV, (const uint8_t*)a.v_pages + byte, full);
+                }
+            }
+            copies_commit();
+        };
+        auto ring_sync = [&]() {
+            if (WR == 1) __syncwarp();
+            else asm volatile("bar.sync %0, %1;" ::"r"(1 + wk), "n"(WR * 32) : "memory");
+        };
+
+        float o[DP / 8][4];
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[i][x] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, mv[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+        look_up(0);
+#pragma unroll
+        for (int t = 0; t < kStages - 1; ++t) {
+            issue(t);
+            look_up(t + 1);
+        }
+        for (int t = 0; t < n; ++t) {
+            copies_wait<kStages - 2>();
+            ring_sync();
+            issue(t + kStages - 1);
+            look_up(t + kStages);
+            const int st = t % kStages;
+            const uint32_t base = ring + st * kStage;
+            const int tile0 = key0 + (r0 + t) * NK;
+#pragma unroll 1
+            for (int kb = 0; kb < TK; kb += KB) {
+                const int first = tile0 + kb;
+                if (first >= rg.total) break;
+                float s[KB / 8][4];
+#pragma unroll
+                for (int i = 0; i < KB / 8; ++i)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[i][x] = 0.f;
+                // scores
+#pragma unroll
+                for (int kp = 0; kp < KB / 16; ++kp) {
+                    const uint32_t krow = base + kK + (kb + kp * 16) * RB;
+                    const int r = ((lane >> 4) << 3) + (lane & 7);
+                    if (E4M3) {
+#pragma unroll
+                        for (int k = 0; k < DP / 16; k += 2) {
+                            uint32_t f[4];
+                            const int ch = (k + ((lane >> 3) & 1)) ^ (r & 7);
+                            ldsm4(f, krow + r * RB + (ch & (CPR - 1)) * 16);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const uint32_t b0 = e4m3x2_to_f16x2(f[x] & 0xffffu), b1 = e4m3x2_to_f16x2(f[x] >> 16);
+                                mma<P>(s[2 * kp + (x >> 1)], q[k + (x & 1)], b0, b1);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < DP / 16; ++k) {
+                            uint32_t f[4];
+                            const int ch = (2 * k + ((lane >> 3) & 1)) ^ (r & 7);
+                            ldsm4(f, krow + r * RB + ch * 16);
+                            mma<P>(s[2 * kp], q[k], f[0], f[1]);
+                            mma<P>(s[2 * kp + 1], q[k], f[2], f[3]);
+                        }
+                    }
+                }
+                float lv[KB / 8][2];  // log2 of the values' scales
+#pragma unroll
+                for (int i = 0; i < KB / 8; ++i) {
+                    float ks0 = 1.f, ks1 = 1.f;
+                    if (E4M3) {
+                        const float* sk = reinterpret_cast<const float*>(smem + (base - smem_addr(smem)) + kSK) + kb + i * 8 + 2 * c;
+                        const float* sv = sk + WR * KW;
+                        ks0 = sk[0];
+                        ks1 = sk[1];
+                        lv[i][0] = __log2f(sv[0]);
+                        lv[i][1] = __log2f(sv[1]);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) s[i][x] *= fac[x >> 1] * ((x & 1) ? ks1 : ks0);
+                }
+                // mask, where a key of this step is hidden from some row
+                const int wsrc = wk * WR + kb / KW;
+                uint32_t valid = s_valid[wsrc][st][LK == 2 ? (kb % KW) / 32 : 0];
+                const uint32_t all_bits = KB == 32 ? 0xffffffffu : 0xffffu;
+                bool hidden = false;
+                if (first + KB - 1 > min_hi || first < max_lo || (valid & all_bits) != all_bits) {
+#pragma unroll
+                    for (int i = 0; i < KB / 8; ++i)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            hidden = true;
+                            const int k = i * 8 + 2 * c + (x & 1), pos = first + k;
+                            if (pos > hi[x >> 1] || pos < lo[x >> 1] || !((valid >> k) & 1)) s[i][x] = -INFINITY;
+                        }
+                }
+                // running maximum (of score + log2 value scale too), rescaling only when some row's grew
+                float tm[2] = {-INFINITY, -INFINITY}, tv[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < KB / 8; ++i)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        tm[x >> 1] = fmaxf(tm[x >> 1], s[i][x]);
+                        if (E4M3) tv[x >> 1] = fmaxf(tv[x >> 1], s[i][x] + lv[i][x & 1]);
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    tm[i] = fmaxf(tm[i], __shfl_xor_sync(0xffffffffu, tm[i], 1));
+                    tm[i] = fmaxf(tm[i], __shfl_xor_sync(0xffffffffu, tm[i], 2));
+                    if (E4M3) {
+                        tv[i] = fmaxf(tv[i], __shfl_xor_sync(0xffffffffu, tv[i], 1));
+                        tv[i] = fmaxf(tv[i], __shfl_xor_sync(0xffffffffu, tv[i], 2));
+                    } else {
+                        tv[i] = tm[i];
+                    }
+                }
+                if (__any_sync(0xffffffffu, tm[0] > m[0] || tm[1] > m[1] || (E4M3 && (tv[0] > mv[0] || tv[1] > mv[1])))) {
+                    float f[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float mn = fmaxf(m[i], tm[i]), vn = fmaxf(mv[i], tv[i]);
+                        l[i] *= m[i] == -INFINITY ? 0.f : exp2f(m[i] - mn);
+                        f[i] = mv[i] == -INFINITY ? 0.f : exp2f(mv[i] - vn);
+                        m[i] = mn;
+                        mv[i] = vn;
+                    }
+#pragma unroll
+                    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[i][x] *= f[x >> 1];
+                }
+                const float mz[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+                const float vz[2] = {mv[0] == -INFINITY ? 0.f : mv[0], mv[1] == -INFINITY ? 0.f : mv[1]};
+                uint32_t p[KB / 16][4];
+#pragma unroll
+                for (int i = 0; i < KB / 8; ++i) {
+                    float e[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const float pr = exp2f(s[i][x] - mz[x >> 1]);
+                        l[x >> 1] += pr;
+                        // a hidden key's scale may be anything
+                        e[x] = !E4M3 ? pr : s[i][x] == -INFINITY ? 0.f : exp2f(s[i][x] + lv[i][x & 1] - vz[x >> 1]);
+                    }
+                    p[i / 2][(i & 1) * 2] = pack2<P>(e[0], e[1]);
+                    p[i / 2][(i & 1) * 2 + 1] = pack2<P>(e[2], e[3]);
+                }
+                // weighted values
+                auto load_values = [&](int kp, int k, uint32_t (&v)[kVal]) {
+                    const uint32_t vrow = base + kV + (kb + kp * 16) * RB;
+                    const int r = (((lane >> 3) & 1) << 3) + (lane & 7);
+                    uint32_t f[4];
+                    const int ch = (k + (lane >> 4)) ^ (r & 7);
+                    ldsm4_t(f, vrow + r * RB + (ch & (CPR - 1)) * 16);
+                    if constexpr (E4M3) {  // even and odd elements of a chunk become two tiles of eight columns
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint32_t u = __byte_perm(f[x], 0, 0x3120);
+                            v[(x >> 1) * 4 + (x & 1)] = e4m3x2_to_f16x2(u & 0xffffu);
+                            v[(x >> 1) * 4 + 2 + (x & 1)] = e4m3x2_to_f16x2(u >> 16);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) v[x] = f[x];
+                    }
+                };
+                if (hidden && M > G && values_not_finite<P, kVal, KB / 16, CPR>(load_values)) {
+                    // A key that some rows see and others do not holds an infinity or a NaN: 0 times it is no 0.  Each token's
+                    // rows get a product of their own in which the keys hidden from them are zeros.
+                    const int last = min(row_base + 15, M - 1) / G;
+                    for (int j = row_base / G; j <= last; ++j) {
+                        const int hj = (int)min((int64_t)rg.start + j, (int64_t)rg.total - 1);
+                        const int lj = a.window > 0 ? (int)max((int64_t)0, (int64_t)rg.start + j + 1 - a.window) : 0;
+#pragma unroll 1
+                        for (int kp = 0; kp < KB / 16; ++kp) {
+                            uint32_t keep[2];
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const int pos = first + kp * 16 + 8 * x + 2 * c;
+                                keep[x] = (pos >= lj && pos <= hj ? 0xffffu : 0u) | (pos + 1 >= lj && pos + 1 <= hj ? 0xffff0000u : 0u);
+                            }
+#pragma unroll
+                            for (int k = 0; k < CPR; k += 2) {
+                                uint32_t v[kVal];
+                                load_values(kp, k, v);
+#pragma unroll
+                                for (int x = 0; x < kVal / 2; ++x) {
+                                    float add[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma<P>(add, p[kp], v[2 * x] & keep[0], v[2 * x + 1] & keep[1]);
+#pragma unroll
+                                    for (int y = 0; y < 4; ++y)
+                                        if (min(row[y >> 1], M - 1) / G == j) o[k * (kVal / 4) + x][y] += add[y];
+                                }
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int kp = 0; kp < KB / 16; ++kp)
+#pragma unroll
+                        for (int k = 0; k < CPR; k += 2) {
+                            uint32_t v[kVal];
+                            load_values(kp, k, v);
+#pragma unroll
+                            for (int x = 0; x < kVal / 2; ++x) mma<P>(o[k * (kVal / 4) + x], p[kp], v[2 * x], v[2 * x + 1]);
+                        }
+                }
+            }
+        }
+        copies_wait<0>();
+
+        // add the rings: every warp leaves its 16 rows in shared memory (rows padded by 4 floats against bank conflicts)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        }
+        __syncthreads();
+        float* mine = reinterpret_cast<float*>(smem) + warp * 16 * (DP + 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            // weighted values are in units of 2^mv: bring them to those of the sum, 2^m
+            const float f = E4M3 ? (mv[i] == -INFINITY ? 0.f : exp2f(mv[i] - m[i])) : 1.f;
+            float* dst = mine + (g + 8 * i) * (DP + 4);
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                if (E4M3) {
+                    *reinterpret_cast<float4*>(dst + k * 16 + 4 * c) =
+                        make_float4(o[2 * k][2 * i] * f, o[2 * k + 1][2 * i] * f, o[2 * k][2 * i + 1] * f, o[2 * k + 1][2 * i + 1] * f);
+                } else {
+                    *reinterpret_cast<float2*>(dst + k * 16 + 2 * c) = make_float2(o[2 * k][2 * i], o[2 * k][2 * i + 1]);
+                    *reinterpret_cast<float2*>(dst + k * 16 + 8 + 2 * c) = make_float2(o[2 * k + 1][2 * i], o[2 * k + 1][2 * i + 1]);
+                }
+            }
+            if (c == 0) {
+                s_ml[warp][g + 8 * i][0] = m[i];
+                s_ml[warp][g + 8 * i][1] = l[i];
+            }
+        }
+        __syncthreads();
+        const bool whole = r0 == 0 && r1 == rg.rounds;
+        const int slot = at == began ? 0 : 1;
+        const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * 16 * WR;
+        const int chunks = a.D / 8;
+        const int tile_base = (item - h * row_tiles) * 16 * WR;
+        const int count = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
+        for (int u = threadIdx.x; u < 16 * WR * chunks; u += 128) {
+            const int r = u / chunks, e = (u - r * chunks) * 8;
+            const int rw = r / 16, rr = r % 16, gr = tile_base + r;
+            if (gr >= M) continue;
+            float top = -INFINITY, sum = 0.f, f[WK], v[8] = {};
+#pragma unroll
+            for (int k = 0; k < WK; ++k) top = fmaxf(top, s_ml[k * WR + rw][rr][0]);
+#pragma unroll
+            for (int k = 0; k < WK; ++k) {
+                const float mk = s_ml[k * WR + rw][rr][0];
+                f[k] = mk == -INFINITY ? 0.f : exp2f(mk - top);
+                // a ring without a finite score has seen nothing, or a NaN that its sum holds
+                sum += mk == -INFINITY ? s_ml[k * WR + rw][rr][1] : f[k] * s_ml[k * WR + rw][rr][1];
+                const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem) + ((k * WR + rw) * 16 + rr) * (DP + 4) + e);
+                const float4 x = src[0], y = src[1];
+                v[0] += f[k] * x.x; v[1] += f[k] * x.y; v[2] += f[k] * x.z; v[3] += f[k] * x.w;
+                v[4] += f[k] * y.x; v[5] += f[k] * y.y; v[6] += f[k] * y.z; v[7] += f[k] * y.w;
+            }
+            if (whole) {
+                const int j = gr / G, hq = h * G + gr - j * G;
+                const float inv = j >= count || sum == 0.f ? 0.f : __fdividef(1.f, sum);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] = j >= count || sum == 0.f ? 0.f : v[x] * inv;
+                *reinterpret_cast<uint4*>((T*)a.out + (((int64_t)b * a.S + j) * a.Hq + hq) * a.D + e) = Vec8<T>::pack(v);
+            } else {
+                float4* dst = reinterpret_cast<float4*>(part_o + (part + r) * a.D + e);
+                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                if (e == 0) {
+                    part_ml[(part + r) * 2] = top;
+                    part_ml[(part + r) * 2 + 1] = sum;
+                }
+            }
+        }
+        at += n;
+        __syncthreads();  // shared memory is refilled by the next piece
+    }
+}
+
+// Adds the pieces of the items that several CTAs of the attention kernel worked on, in their order along the keys.
+template <typename T>
+__global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int B, int NK, int rows, int ctas, const float* __restrict__ part_ml,
+                                                   const float* __restrict__ part_o) {
+    __shared__ int64_t scratch[8];
+    const int b = blockIdx.y, item = blockIdx.x;
+    const int G = a.Hq / a.Hkv, M = a.S * G, row_tiles = (M + rows - 1) / rows;
+    const int64_t per = (int64_t)a.Hkv * row_tiles;
+    int64_t before, all;
+    sum_rounds(a, B, NK, b, before, all, scratch);
+    const Range rg = seq_range(a, b, NK);
+    all *= per;
+    const int64_t s = before * per + (int64_t)item * rg.rounds, e = s + rg.rounds;
+    const int64_t c0 = ((s + 1) * ctas - 1) / all, c1 = (e * ctas - 1) / all;
+    if (c0 == c1) return;
+    const int h = item / row_tiles, tile_base = (item - h * row_tiles) * rows;
+    const int count = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
+    const int chunks = a.Dv / 4;
+    for (int u = threadIdx.x; u < rows * chunks; u += 128) {
+        const int r = u / chunks, x = (u - r * chunks) * 4, gr = tile_base + r;
+        if (gr >= M) break;
+        float top = -INFINITY, sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int64_t c = c0; c <= c1; ++c) {
+            const int64_t begin = c * all / ctas;
+            if (begin == (c + 1) * all / ctas) continue;  // a CTA without work
+            const int64_t part = (c * 2 + (begin >= s ? 0 : 1)) * rows + r;
+            const float m = part_ml[part * 2], l = part_ml[part * 2 + 1];
+            const float mn = fmaxf(top, m);
+            const float f0 = top == -INFINITY ? 0.f : exp2f(top - mn), f1 = m == -INFINITY ? 0.f : exp2f(m - mn);
+            const float4 o = *reinterpret_cast<const float4*>(part_o + part * a.Dv + x);
+            sum = (top == -INFINITY ? sum : sum * f0) + (m == -INFINITY ? l : l * f1);
+            v.x = v.x * f0 + o.x * f1;
+            v.y = v.y * f0 + o.y * f1;
+            v.z = v.z * f0 + o.z * f1;
+            v.w = v.w * f0 + o.w * f1;
+            top = mn;
+        }
+        const int j = gr / G, hq = h * G + gr - j * G;
+        const bool none = j >= count || sum == 0.f;
+        const float inv = __fdividef(1.f, sum);
+        uint2 res;
+        res.x = none ? 0u : pack2<T>(v.x * inv, v.y * inv);
+        res.y = none ? 0u : pack2<T>(v.z * inv, v.w * inv);
+        *reinterpret_cast<uint2*>((T*)a.out + (((int64_t)b * a.S + j) * a.Hq + hq) * a.Dv + x) = res;
+    }
+}
+
+// once per kernel and device
+template <typename K>
+static void allow_smem_once(K kernel, int bytes, std::atomic<uint64_t>& done) {
+    const int dev = at::cuda::current_device();
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return;
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+}
+
+template <typename T, bool E4M3, int DP, int WR>
+static void launch_rows(const AttnArgs& a, int64_t B, const at::Tensor& q) {
+    using Sh = Shape<E4M3, DP>;
+    static std::atomic<uint64_t> done{0};
+    allow_smem_once(rows_kernel<T, E4M3, DP, WR>, Sh::kSmem, done);
+    const int rows = 16 * WR, ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount * (Sh::kSmem > 110000 ? 1 : 2);
+    const int G = a.Hq / a.Hkv;
+    const int64_t row_tiles = ceil_div((int64_t)a.S * G, rows), items = a.Hkv * row_tiles;
+    ATB_ARG(items < (int64_t(1) << 31) && B <= 65535, "paged_attention: too many query rows or sequences");
+    const at::Tensor ws = at::empty({(int64_t)ctas * 2 * rows * (a.Dv + 2)}, q.options().dtype(at::kFloat));
+    float* part_o = ws.data_ptr<float>();
+    float* part_ml = part_o + (int64_t)ctas * 2 * rows * a.Dv;
+    cudaStream_t st = current_stream();
+    rows_kernel<T, E4M3, DP, WR><<<ctas, 128, Sh::kSmem, st>>>(a, (int)B, part_ml, part_o);
+    ATB_LAUNCH_CHECK();
+    join_kernel<T><<<dim3((unsigned)items, (unsigned)B), 128, 0, st>>>(a, (int)B, Sh::kRound, rows, ctas, part_ml, part_o);
+    ATB_LAUNCH_CHECK();
+}
+
+template <typename T, bool E4M3, int DP>
+static void launch_heads(const AttnArgs& a, int64_t B, const at::Tensor& q) {
+    const int rows = a.S * (a.Hq / a.Hkv);
+    if (rows <= 16) launch_rows<T, E4M3, DP, 1>(a, B, q);
+    else if (rows <= 32) launch_rows<T, E4M3, DP, 2>(a, B, q);
+    else launch_rows<T, E4M3, DP, 4>(a, B, q);
+}
+
+template <typename T, bool E4M3>
+static void launch_dims(const AttnArgs& a, int64_t B, const at::Tensor& q) {
+    if (a.D <= 64) launch_heads<T, E4M3, 64>(a, B, q);
+    else if (a.D <= 128) launch_heads<T, E4M3, 128>(a, B, q);
+    else launch_heads<T, E4M3, 256>(a, B, q);
+}
+
+// ---- latent attention --------------------------------------------------------------------------------------------------
 template <typename T, bool E4M3>
 __device__ __forceinline__ void load8(const void* base, int64_t at, float (&f)[8]) {
     if (E4M3) unpack_e4m3x8(*reinterpret_cast<const uint2*>((const uint8_t*)base + at), f);
@@ -143,6 +857,8 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const
     check_pages(op, k_pages, k_scale, q);
     check_pages(op, v_pages, v_scale, q);
     ATB_ARG(k_pages.sizes() == v_pages.sizes() && k_pages.scalar_type() == v_pages.scalar_type(), op, ": k_pages and v_pages differ");
+    ATB_ARG(k_pages.stride(0) == v_pages.stride(0) && (!k_scale.has_value() || k_scale->stride(0) == v_scale->stride(0)), op,
+            ": the pages of keys and values must lie equally far apart");
     const int64_t Hkv = k_pages.size(1);
     ATB_ARG(Hkv > 0 && Hq % Hkv == 0, op, ": the query heads must be a multiple of the cache's heads");
     ATB_ARG(k_pages.size(3) == D, op, ": the cache has another dim than q");
@@ -153,6 +869,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const
     const c10::cuda::CUDAGuard guard(q.device());
     at::Tensor out = at::empty({B, S, Hq, D}, q.options());
     if (out.numel() == 0) return out;
+    if (k_pages.size(0) == 0 || table.size(1) == 0) return out.zero_();
     const at::Tensor qc = rows16(q);
     AttnArgs a;
     a.q = qc.data_ptr(); a.q2 = nullptr;
@@ -166,7 +883,9 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const
     a.table_stride = table.stride(0);
     a.S = (int)S; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.D = a.D1 = a.Dv = (int)D; a.P = (int)k_pages.size(0); a.W = (int)table.size(1);
     a.page = (int)k_pages.size(2); a.window = (int)window; a.scale = (float)scale;
-    launch_attention(q, is_e4m3(k_pages), a, B);
+    const bool f8 = is_e4m3(k_pages);
+    if (q.scalar_type() == at::kBFloat16) f8 ? launch_dims<bf16, true>(a, B, q) : launch_dims<bf16, false>(a, B, q);
+    else f8 ? launch_dims<__half, true>(a, B, q) : launch_dims<__half, false>(a, B, q);
     return out;
 }
 
@@ -189,6 +908,7 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& q_pe, c
     const c10::cuda::CUDAGuard guard(q.device());
     at::Tensor out = at::empty({B, S, H, R}, q.options());
     if (out.numel() == 0) return out;
+    if (pages.size(0) == 0 || table.size(1) == 0) return out.zero_();
     const at::Tensor qc = rows16(q), pc = rows16(q_pe);
     AttnArgs a;
     a.q = qc.data_ptr(); a.q2 = pc.data_ptr();

@@ -315,7 +315,13 @@ def _paged_softmax_product(q, k, v, held, starts, counts, scale: float, window) 
     scores = torch.matmul(qf, k.unsqueeze(2).transpose(-1, -2)) * scale
     scores = scores.masked_fill(~seen.view(B, 1, 1, S, L), float("-inf"))
     p = torch.softmax(scores, dim=-1).masked_fill(~seen.any(-1).view(B, 1, 1, S, 1), 0.0)
-    return torch.matmul(p, v.unsqueeze(2)).permute(0, 3, 1, 2, 4).reshape(B, S, Hq, -1).to(q.dtype)
+    finite = torch.isfinite(v)
+    o = torch.matmul(p, torch.where(finite, v, 0.0).unsqueeze(2))
+    # infinities and NaN reach the queries that see them, and no others (0 times them is no 0)
+    for t in torch.nonzero(~finite.all(-1).all(1).all(0)).flatten().tolist():
+        rest = torch.where(finite[:, :, t], 0.0, v[:, :, t]).view(B, Hkv, 1, 1, -1)
+        o = o + torch.where(seen[:, :, t].view(B, 1, 1, S, 1), p[..., t : t + 1] * rest, 0.0)
+    return o.permute(0, 3, 1, 2, 4).reshape(B, S, Hq, -1).to(q.dtype)
 
 
 def paged_attention(q, k_pages, v_pages, page_table, starts, counts, k_scale, v_scale, scale: float, window) -> torch.Tensor:

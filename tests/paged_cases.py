@@ -214,3 +214,39 @@ def refusals(device, dtype):
         "read: lengths of longs": read(s=su.starts.long()),
         "read: table of 1 dim": read(t=su.table[0]),
     }
+
+
+def not_finite_case(dtype, e4m3, device, latent=False, window=None):
+    """A draft whose third token has a NaN key, an infinite value and a NaN value in some places: earlier queries (and, with a
+    window, later ones that no longer see it) must not notice.  e4m3 rows hold a NaN scale instead."""
+    c = dict(starts=[20, 70], S=5, hq=8, hkv=1 if latent else 2, page=16)
+    D, R = (576, 512) if latent else (64, None)
+    su = set_up(c, dtype, e4m3, device, values=not latent, d=D)
+    for b in range(2):
+        p = su.starts_list[b] + 2
+        pid, off = su.table_list[b][p // 16], p % 16
+        if e4m3:
+            (su.k_scale if latent else su.v_scale)[pid, 0, off] = float("nan")
+        else:
+            pages = su.k_pages if latent else su.v_pages
+            pages[pid, 0, off, 3] = float("inf")
+            pages[pid, 0, off, 8] = float("nan")
+            if not latent:
+                su.k_pages[pid, 1, off, 5] = float("nan")
+    scale = 0.1
+    if latent:
+        q, q_pe = su.normal(2, 5, 8, R), su.normal(2, 5, 8, D - R)
+        got = ops.paged_latent_attention(q, q_pe, su.k_pages, su.table, su.starts, None, su.k_scale, scale)
+        want, tol = po.attention(su, torch.cat((q, q_pe), -1), scale, latent=R, p_type=p_type(dtype, e4m3))
+    else:
+        q = su.normal(2, 5, 8, D)
+        got = ops.paged_attention(q, su.k_pages, su.v_pages, su.table, su.starts, None, su.k_scale, su.v_scale, scale, window)
+        want, tol = po.attention(su, q, scale, window, p_type=p_type(dtype, e4m3))
+    assert torch.isfinite(want[:, :2]).all() and not torch.isfinite(want[:, 2]).all()
+    if window == 2:
+        assert torch.isfinite(want[:, 4]).all()
+    got = got.cpu().double()
+    fine = torch.isfinite(want)
+    assert torch.equal(fine, torch.isfinite(got))
+    po.check_close(torch.where(fine, got, 0.0), torch.where(fine, want, 0.0),
+                   torch.where(fine, tol * 1.01 + want.abs() * po.step(dtype) * 1.02 + po.floor(dtype), 0.0), "not finite")

@@ -40,6 +40,17 @@ def test_read(name, dtype, e4m3):
     pc.read_case(pc.ATTENTION[name], dtype, e4m3, "cpu", values=name != "ragged")
 
 
+@pytest.mark.parametrize("window", [None, 2])
+@pytest.mark.parametrize("dtype,e4m3", TYPES, ids=str)
+def test_hidden_values_that_are_not_finite(dtype, e4m3, window):
+    pc.not_finite_case(dtype, e4m3, "cpu", window=window)
+
+
+@pytest.mark.parametrize("dtype,e4m3", TYPES, ids=str)
+def test_hidden_latents_that_are_not_finite(dtype, e4m3):
+    pc.not_finite_case(dtype, e4m3, "cpu", latent=True)
+
+
 @pytest.mark.parametrize("dtype", [pc.F32, pc.BF], ids=str)
 @pytest.mark.parametrize("name", list(pc.refusals("cpu", pc.F32)))
 def test_refusals(name, dtype):

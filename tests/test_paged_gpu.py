@@ -61,6 +61,17 @@ def test_latent_attention(name, dtype, e4m3):
     pc.latent_case(pc.LATENT[name], dtype, e4m3, "cuda")
 
 
+@pytest.mark.parametrize("window", [None, 2])
+@pytest.mark.parametrize("dtype,e4m3", TYPES, ids=str)
+def test_hidden_values_that_are_not_finite(dtype, e4m3, window):
+    pc.not_finite_case(dtype, e4m3, "cuda", window=window)
+
+
+@pytest.mark.parametrize("dtype,e4m3", TYPES, ids=str)
+def test_hidden_latents_that_are_not_finite(dtype, e4m3):
+    pc.not_finite_case(dtype, e4m3, "cuda", latent=True)
+
+
 @pytest.mark.parametrize("shape", [(0, 1, 4, 2), (2, 0, 4, 2), (2, 1, 0, 2)])
 def test_empty_calls(shape):
     B, S, hq, hkv = shape
@@ -80,3 +91,107 @@ def test_no_pages():
     full = torch.ones(2, 2, 16, 32, device="cuda", dtype=pc.BF)
     assert torch.equal(ops.paged_attention(q, full, full, table[:, :0], starts), torch.zeros_like(q))
     assert torch.equal(ops.paged_kv_read(pages, None, table, starts, 5)[0], torch.zeros(2, 5, 2, 32, device="cuda", dtype=pc.BF))
+
+
+def _attention_inputs(starts, S=1, hq=16, hkv=4, d=128, e4m3=False, seed=0):
+    su = pc.set_up(dict(starts=starts, S=S, page=16), pc.BF, e4m3, "cuda", d=d, hkv=hkv, seed=seed)
+    return su, su.normal(su.B, S, hq, d)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_same_bits_every_time(e4m3):
+    su, q = _attention_inputs([5000, 17, 1234, 900], e4m3=e4m3)
+    args = (su.k_pages, su.v_pages, su.table, su.starts, None, su.k_scale, su.v_scale)
+    first = ops.paged_attention(q, *args)
+    for _ in range(5):
+        assert torch.equal(ops.paged_attention(q, *args).view(torch.int16), first.view(torch.int16))
+
+
+def test_two_captured_graphs_replayed_in_turn():
+    """Each graph has a workspace of its own, and reads the lengths and pages of the moment it is replayed."""
+    sets = [_attention_inputs([3000, 40], seed=1), _attention_inputs([700, 2500, 9], seed=2)]
+
+    def call(i):
+        su, q = sets[i]
+        return ops.paged_attention(q, su.k_pages, su.v_pages, su.table, su.starts)
+
+    want = [call(0), call(1)]
+    graphs, outs = [], []
+    for i in range(2):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call(i)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(i)
+        graphs.append(graph)
+        outs.append(out)
+    for _ in range(3):
+        for i in range(2):
+            outs[i].zero_()
+        graphs[0].replay()
+        graphs[1].replay()
+        for i in range(2):
+            assert torch.equal(outs[i], want[i])
+    su, q = sets[0]
+    su.starts.fill_(39)
+    graphs[0].replay()
+    assert torch.equal(outs[0], call(0)) and not torch.equal(outs[0], want[0])
+
+
+def test_two_streams_at_once():
+    sets = [_attention_inputs([4000, 300], seed=3), _attention_inputs([2000, 3000, 1], seed=4)]
+    want = [ops.paged_attention(q, su.k_pages, su.v_pages, su.table, su.starts) for su, q in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i, (su, q) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.paged_attention(q, su.k_pages, su.v_pages, su.table, su.starts))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_a_strided_query_and_pages_of_one_tensor():
+    """Queries as a view of a projection output, misaligned queries, and keys and values that share one allocation."""
+    su, q = _attention_inputs([333, 90])
+    want = ops.paged_attention(q, su.k_pages, su.v_pages, su.table, su.starts)
+    wide = torch.randn(2, 1, 40 * 128, device="cuda").to(pc.BF)
+    wide[..., : 16 * 128] = q.reshape(2, 1, -1)
+    view = wide[..., : 16 * 128].unflatten(-1, (16, 128))
+    odd = torch.empty(q.numel() + 1, device="cuda", dtype=pc.BF)[1:].view(q.shape).copy_(q)
+    both = torch.stack([su.k_pages, su.v_pages], 1)
+    table = torch.cat([su.table, torch.full_like(su.table, -7)], 1)[:, : su.W]
+    for args in ((view, su.k_pages, su.v_pages, su.table), (odd, su.k_pages, su.v_pages, su.table), (q, both[:, 0], both[:, 1], table)):
+        assert torch.equal(ops.paged_attention(*args, su.starts), want)
+
+
+def test_pages_shared_by_sequences():
+    """Two sequences with a common prefix read the same pages."""
+    su, q = _attention_inputs([100, 100])
+    table = su.table.clone()
+    table[1, :5] = table[0, :5]
+    got = ops.paged_attention(q, su.k_pages, su.v_pages, table, su.starts)
+    su.table_list = table.tolist()
+    po.check_attention(got, *po.attention(su, q, 128**-0.5, p_type=pc.BF))
+
+
+def test_a_cache_of_more_than_2_31_elements():
+    """Offsets past 2^31 elements (and 2^32 bytes): the last page of a large pool."""
+    n = (2**31 + 2**20) // (2 * 64 * 128)
+    pages = torch.zeros(n, 2, 64, 128, device="cuda", dtype=pc.BF)
+    pages[-1].normal_()
+    table = torch.tensor([[n - 1]], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([63], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 1, 8, 128, device="cuda").to(pc.BF)
+    small = pages[-1:].clone()
+    assert torch.equal(ops.paged_attention(q, pages, pages, table, starts),
+                       ops.paged_attention(q, small, small, torch.zeros_like(table), starts))
+    got, _ = ops.paged_kv_read(pages, None, table, starts, 63)
+    assert torch.equal(got[0], small[0, :, :63].transpose(0, 1))
+    kv, cos, sin = torch.randn(1, 1, 2, 128, device="cuda").to(pc.BF), torch.ones(1, 1, 64, device="cuda"), torch.zeros(1, 1, 64, device="cuda")
+    ops.paged_kv_append(q, kv, kv, cos, sin, pages, pages, table, starts - 3)
+    assert torch.equal(pages[-1, :, 60], kv[0, 0])
