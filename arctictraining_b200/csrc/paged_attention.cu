@@ -27,10 +27,12 @@ struct AttnArgs {
 
 // ---- schedule ---------------------------------------------------------------------------------------------------------
 // Work is counted in rounds of `NK` keys of one item (sequence, cache head, tile of query rows).  The rounds of all items
-// stand in one line and every CTA takes an equal piece of it, so a batch of very different lengths loads all SMs alike
+// stand in one line, each item's behind kLead empty ones that stand for what an item costs besides its keys (its queries,
+// the pipeline's filling, the result: 2 to 3 us, a round 1.5 to 2 us), and every CTA takes an equal piece of the line, so a batch of very different lengths loads all SMs alike
 // and a single long sequence is spread over all of them.  A CTA that covers an item alone writes the result; otherwise it
 // leaves (maximum, sum, weighted values) of its piece in the workspace, and the join kernel adds the pieces in their
 // order.  No atomics: the same inputs give the same bits.
+constexpr int kLead = 2;
 struct Range {  // the cached positions that the queries of one sequence see
     int start, total, low, first, rounds;  // positions [low, total); counted from `first`, a multiple of NK
 };
@@ -42,23 +44,31 @@ __device__ __forceinline__ Range seq_range(const AttnArgs& a, int b, int NK) {
     r.total = count == 0 ? 0 : (int)max((int64_t)0, min(end, cap));
     r.low = a.window > 0 ? (int)max((int64_t)0, min((int64_t)r.start + 1 - a.window, (int64_t)r.total)) : 0;
     r.first = r.low / NK * NK;
-    r.rounds = max(1, (r.total - r.first + NK - 1) / NK);  // a sequence that sees nothing has one round, fully masked
+    r.rounds = kLead + max(1, (r.total - r.first + NK - 1) / NK);  // a sequence that sees nothing has one round, fully masked
     return r;
 }
 
-// Sum of the rounds of the sequences before `upto`, and of all: by a CTA of 128 threads.
-__device__ __forceinline__ void sum_rounds(const AttnArgs& a, int B, int NK, int upto, int64_t& before, int64_t& all, int64_t* scratch) {
-    int64_t x = 0, y = 0;
+// How `all` rounds are divided: the first `rest` CTAs take one more than the others.  (32-bit: the host bounds the line.)
+struct Pieces {
+    int share, rest;
+    __device__ __forceinline__ Pieces(int all, int ctas) : share(all / ctas), rest(all - all / ctas * ctas) {}
+    __device__ __forceinline__ int begin(int cta) const { return cta * share + min(cta, rest); }
+    __device__ __forceinline__ int cta_of(int round) const {
+        const int wide = rest * (share + 1);
+        return round < wide ? round / (share + 1) : rest + (round - wide) / max(share, 1);
+    }
+};
+
+// Rounds of the sequences before `upto`, and of all: by a CTA of 128 threads.
+__device__ __forceinline__ void sum_rounds(const AttnArgs& a, int B, int NK, int upto, int& before, int& all, int* scratch) {
+    int x = 0, y = 0;
     for (int b = threadIdx.x; b < B; b += 128) {
         const int n = seq_range(a, b, NK).rounds;
         y += n;
         if (b < upto) x += n;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, o);
-        y += __shfl_xor_sync(0xffffffffu, y, o);
-    }
+    x = __reduce_add_sync(0xffffffffu, x);
+    y = __reduce_add_sync(0xffffffffu, y);
     if ((threadIdx.x & 31) == 0) {
         scratch[threadIdx.x >> 5] = x;
         scratch[4 + (threadIdx.x >> 5)] = y;
@@ -68,47 +78,46 @@ __device__ __forceinline__ void sum_rounds(const AttnArgs& a, int B, int NK, int
     all = scratch[4] + scratch[5] + scratch[6] + scratch[7];
 }
 
-// The sequence that holds round `at` of the line (every sequence has `per` items), and its first round.
-__device__ __forceinline__ void find_round(const AttnArgs& a, int B, int NK, int64_t per, int64_t at, int& b_out, int64_t& first_out,
-                                           int64_t& all, int64_t* scratch) {
+// This CTA's piece [at, to) of the line, the sequence that holds its first round (a sequence has `per` items) and that
+// sequence's first round.
+__device__ __forceinline__ void find_piece(const AttnArgs& a, int B, int NK, int per, int& at, int& to, int& b_out, int& line, int* scratch) {
     // thread i looks at sequences [i n, (i + 1) n)
     const int n = (B + 127) / 128, b0 = threadIdx.x * n, b1 = min(B, b0 + n);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t mine = 0;
+    int mine = 0;
     for (int b = b0; b < b1; ++b) mine += seq_range(a, b, NK).rounds;
-    int64_t incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
     }
     if (lane == 31) scratch[warp] = incl;
     __syncthreads();
-    int64_t base = 0;
-    all = 0;
+    int base = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         if (w < warp) base += scratch[w];
         all += scratch[w];
     }
-    all *= per;
-    int64_t lo = (base + incl - mine) * per;
-    // `at` is given as a fraction of the line: CTA c starts at c * all / CTAs
-    const int64_t target = at * all / gridDim.x;
-    if (target >= lo && target < lo + mine * per) {
+    const Pieces pieces(all * per, gridDim.x);
+    at = pieces.begin(blockIdx.x);
+    to = pieces.begin(blockIdx.x + 1);
+    int lo = (base + incl - mine) * per;
+    if (at < to && at >= lo && at < lo + mine * per) {
         int b = b0;
         while (true) {
-            const int64_t r = (int64_t)seq_range(a, b, NK).rounds * per;
-            if (target < lo + r) break;
+            const int r = seq_range(a, b, NK).rounds * per;
+            if (at < lo + r) break;
             lo += r;
             ++b;
         }
-        scratch[8] = b;
-        scratch[9] = lo;
+        scratch[4] = b;
+        scratch[5] = lo;
     }
     __syncthreads();
-    b_out = (int)scratch[8];
-    first_out = scratch[9];
+    b_out = scratch[4];
+    line = scratch[5];
 }
 
 // ---- tensor-core pieces -----------------------------------------------------------------------------------------------
@@ -216,7 +225,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
     constexpr int KB = KW < 32 ? KW : 32;  // keys of one softmax step
     constexpr int kVal = E4M3 ? 8 : 4;     // registers of two 16-byte chunks of 16 values
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t scratch[16];
+    __shared__ int scratch[8];
     __shared__ uint32_t s_valid[4][kStages][2];
     __shared__ float s_ml[4][16][2];
 
@@ -225,15 +234,13 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
     const int g = lane >> 2, c = lane & 3;
     const int G = a.Hq / a.Hkv, M = a.S * G;
     const int row_tiles = (M + 16 * WR - 1) / (16 * WR);
-    const int64_t per = (int64_t)a.Hkv * row_tiles;
+    const int per = a.Hkv * row_tiles;
 
-    int b;
-    int64_t line, all;
-    find_round(a, B, NK, per, blockIdx.x, b, line, all, scratch);
-    int64_t at = (int64_t)blockIdx.x * all / gridDim.x;
-    const int64_t to = ((int64_t)blockIdx.x + 1) * all / gridDim.x;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join kernel may be set up meanwhile
+    int b, line, at, to;
+    find_piece(a, B, NK, per, at, to, b, line, scratch);
     if (at >= to) return;
-    const int64_t began = at;
+    const int began = at;
     Range rg = seq_range(a, b, NK);
 
     const uint32_t ring = smem_addr(smem) + wk * WR * kStages * Sh::kStageBytes;
@@ -246,10 +253,13 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
             ++b;
             rg = seq_range(a, b, NK);
         }
-        const int64_t in_seq = at - line;
-        const int item = (int)(in_seq / rg.rounds);  // (cache head, row tile)
-        const int r0 = (int)(in_seq - (int64_t)item * rg.rounds);
-        const int r1 = (int)min((int64_t)rg.rounds, r0 + (to - at));
+        const int item = (at - line) / rg.rounds;  // (cache head, row tile)
+        const int v0 = at - line - item * rg.rounds, v1 = min(rg.rounds, v0 + (to - at));
+        const int r0 = max(0, v0 - kLead), r1 = v1 - kLead;
+        if (r1 <= r0) {  // only empty rounds of the item
+            at += v1 - v0;
+            continue;
+        }
         const int h = item / row_tiles, row_base = (item - h * row_tiles) * 16 * WR + wr * 16;
 
         // query rows of this lane, and the positions that they see
@@ -277,7 +287,16 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
                     q[k][i + 2] = in ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8 + 2 * c) : 0u;
                 }
             }
-            fac[i] = a.scale * kLog2e;
+            // scores are multiplied by |scale| log2 e; a negative scale turns the queries' signs, and one of zero becomes tiny
+            // so that a hidden key's -infinity stays what it is
+            fac[i] = fmaxf(fabsf(a.scale), 1e-30f) * kLog2e;
+            if (a.scale < 0.f) {
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    q[k][i] ^= 0x80008000u;
+                    q[k][i + 2] ^= 0x80008000u;
+                }
+            }
         }
         if (E4M3 && std::is_same<T, bf16>::value) {
             // bf16 queries become fp16 after a power of two per row that brings their largest element to [2^14, 2^15):
@@ -314,49 +333,110 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
         const int key0 = rg.first + wk * TK;  // of the ring's tile in round 0 of the item
         const int n = r1 - r0;
         const int64_t head_rows = (int64_t)h * a.page;
-        // page of the key that this lane looks up for tile t (KW keys a warp; lanes beyond them idle; 64 keys: two a lane)
+        // Copies of one tile.  `even`: the keys that a warp loads lie in one page and rows are as wide as the stage's, so the
+        // tile is one dense block; otherwise each lane looks up the page of its own key (64 keys: two) and the copies fetch
+        // their row's place from it.  Positions advance by NK a tile: page and offset are carried along without a division.
+        // The page id of the next tile is read a tile ahead.
         constexpr int LK = KW > 32 ? 2 : 1;
-        int pid_next[LK];
-        auto look_up = [&](int t) {
+        const bool even = a.page % KW == 0 && a.D == DP;
+        const int step_w = NK / a.page, step_off = NK - step_w * a.page;
+        int look_key[LK], look_w[LK], look_off[LK], pid_next[LK];
+#pragma unroll
+        for (int x = 0; x < LK; ++x) {
+            look_key[x] = key0 + r0 * NK + wr * KW + (even ? 0 : lane + 32 * x);
+            look_w[x] = look_key[x] / a.page;
+            look_off[x] = look_key[x] - look_w[x] * a.page;
+        }
+        const int* table = a.table + b * a.table_stride;
+        auto look_up = [&](int t) {  // the page ids of tile t, whose positions look_* hold
 #pragma unroll
             for (int x = 0; x < LK; ++x) {
-                const int key = key0 + (r0 + t) * NK + wr * KW + lane + 32 * x;
                 pid_next[x] = -1;
-                if (t < n && (KW >= 32 || lane < KW) && key >= rg.low && key < rg.total) pid_next[x] = a.table[b * a.table_stride + key / a.page];
+                const bool mine = even ? look_key[x] + KW > rg.low : (KW >= 32 || lane < KW) && look_key[x] >= rg.low;
+                if (t < n && mine && look_key[x] < rg.total) pid_next[x] = table[look_w[x]];
             }
         };
-        auto issue = [&](int t) {  // the copies of tile t of this piece
+        auto issue = [&](int t) {  // the copies of tile t of this piece; look_* and pid_next are its, and move on to the next
             if (t < n) {
                 const int st = t % kStages;
                 const uint32_t base = ring + st * kStage;
-                int64_t off[LK];
-                bool ok[LK];
+                constexpr int kIter = KW * CPR / 32;
+                if (even) {
+                    const int pid = pid_next[0], upto = rg.total - look_key[0], from = rg.low - look_key[0];
+                    const bool ok = pid >= 0 && pid < a.P;
+                    const int64_t r = head_rows + look_off[0];
+                    const int64_t off = (ok ? pid * a.k_page + r * DP : 0) * (E4M3 ? 1 : 2) + lane * 16;
+                    const uint8_t *ks = (const uint8_t*)a.k_pages + off, *vs = (const uint8_t*)a.v_pages + off;
+                    // row i * 32 / CPR + lane / CPR: its chunk's place is exchanged within the row by the row's low bits
+                    const int key = lane / CPR, ch = lane % CPR;
+                    const uint32_t d = base + (wr * KW + key) * RB;
+                    if (ok && upto >= KW && from <= 0) {
 #pragma unroll
-                for (int x = 0; x < LK; ++x) {
-                    const int key = key0 + (r0 + t) * NK + wr * KW + lane + 32 * x;
-                    ok[x] = pid_next[x] >= 0 && pid_next[x] < a.P;
-                    const int64_t r = head_rows + key % a.page;
-                    off[x] = ok[x] ? pid_next[x] * a.k_page + r * a.D : 0;
-                    const uint32_t bits = __ballot_sync(0xffffffffu, ok[x]);
-                    if (lane == 0) s_valid[warp][st][x] = bits;
-                    if (E4M3 && (KW >= 32 || lane < KW)) {
-                        const int64_t so = ok[x] ? pid_next[x] * a.ks_page + r : 0;
-                        const uint32_t d = base + kSK + (wr * KW + lane + 32 * x) * 4;
-                        copy4(d, a.k_scale + so, ok[x]);
-                        copy4(d + (kSV - kSK), a.v_scale + so, ok[x]);
+                        for (int i = 0; i < kIter; ++i) {
+                            const uint32_t di = d + i * 512 + ((ch ^ key ^ (i * (32 / CPR) & 7)) & (CPR - 1)) * 16;
+                            copy16(di + kK, ks + i * 512, true);
+                            copy16(di + kV, vs + i * 512, true);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kIter; ++i) {
+                            const int k = i * (32 / CPR) + key;
+                            const bool full = ok && k >= from && k < upto;
+                            const uint32_t di = d + i * 512 + ((ch ^ key ^ (i * (32 / CPR) & 7)) & (CPR - 1)) * 16;
+                            copy16(di + kK, full ? ks + i * 512 : a.k_pages, full);
+                            copy16(di + kV, full ? vs + i * 512 : a.v_pages, full);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < LK; ++x) {
+                        const int k = lane + 32 * x;
+                        const bool full = ok && k >= from && k < upto;
+                        if (E4M3 && k < KW) {
+                            const int64_t so = full ? pid * a.ks_page + r + k : 0;
+                            copy4(base + kSK + (wr * KW + k) * 4, a.k_scale + so, full);
+                            copy4(base + kSV + (wr * KW + k) * 4, a.v_scale + so, full);
+                        }
+                        const uint32_t bits = __ballot_sync(0xffffffffu, full);
+                        if (lane == 0) s_valid[warp][st][x] = bits;
+                    }
+                } else {
+                    int64_t off[LK];
+                    bool ok[LK];
+#pragma unroll
+                    for (int x = 0; x < LK; ++x) {
+                        ok[x] = pid_next[x] >= 0 && pid_next[x] < a.P;
+                        const int64_t r = head_rows + look_off[x];
+                        off[x] = ok[x] ? pid_next[x] * a.k_page + r * a.D : 0;
+                        const uint32_t bits = __ballot_sync(0xffffffffu, ok[x]);
+                        if (lane == 0) s_valid[warp][st][x] = bits;
+                        if (E4M3 && (KW >= 32 || lane < KW)) {
+                            const int64_t so = ok[x] ? pid_next[x] * a.ks_page + r : 0;
+                            const uint32_t d = base + kSK + (wr * KW + lane + 32 * x) * 4;
+                            copy4(d, a.k_scale + so, ok[x]);
+                            copy4(d + (kSV - kSK), a.v_scale + so, ok[x]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kIter; ++i) {
+                        const int id = i * 32 + lane, key = id / CPR, ch = id % CPR;
+                        const int64_t o = __shfl_sync(0xffffffffu, LK == 2 && i * 32 / CPR >= 32 ? off[LK - 1] : off[0], key & 31);
+                        const bool full = __shfl_sync(0xffffffffu, LK == 2 && i * 32 / CPR >= 32 ? ok[LK - 1] : ok[0], key & 31) &&
+                                          ch * 16 < a.D * (E4M3 ? 1 : 2);
+                        const int64_t byte = full ? (E4M3 ? o : o * 2) + ch * 16 : 0;
+                        const uint32_t d = base + (wr * KW + key) * RB + ((ch ^ (key & 7)) & (CPR - 1)) * 16;
+                        copy16(d + kK, (const uint8_t*)a.k_pages + byte, full);
+                        copy16(d + kV, (const uint8_t*)a.v_pages + byte, full);
                     }
                 }
-                constexpr int kIter = KW * CPR / 32;
 #pragma unroll
-                for (int i = 0; i < kIter; ++i) {
-                    const int id = i * 32 + lane, key = id / CPR, ch = id % CPR;
-                    const int64_t o = __shfl_sync(0xffffffffu, LK == 2 && i * 32 / CPR >= 32 ? off[LK - 1] : off[0], key & 31);
-                    const bool full = __shfl_sync(0xffffffffu, LK == 2 && i * 32 / CPR >= 32 ? ok[LK - 1] : ok[0], key & 31) &&
-                                      ch * 16 < a.D * (E4M3 ? 1 : 2);
-                    const int64_t byte = full ? (E4M3 ? o : o * 2) + ch * 16 : 0;
-                    const uint32_t d = base + (wr * KW + key) * RB + ((ch ^ (key & 7)) & (CPR - 1)) * 16;
-                    copy16(d + kK, (const uint8_t*)a.k_pages + byte, full);
-                    copy16(d + kV, (const uint8_t*)a.v_pages + byte, full);
+                for (int x = 0; x < LK; ++x) {
+                    look_key[x] += NK;
+                    look_w[x] += step_w;
+                    look_off[x] += step_off;
+                    if (look_off[x] >= a.page) {
+                        look_off[x] -= a.page;
+                        ++look_w[x];
+                    }
                 }
             }
             copies_commit();
@@ -409,7 +489,8 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
                             ldsm4(f, krow + r * RB + (ch & (CPR - 1)) * 16);
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
-                                const uint32_t b0 = e4m3x2_to_f16x2(f[x] & 0xffffu), b1 = e4m3x2_to_f16x2(f[x] >> 16);
+                                uint32_t b0, b1;
+                                e4m3x4_to_f16x4(f[x], b0, b1);
                                 mma<P>(s[2 * kp + (x >> 1)], q[k + (x & 1)], b0, b1);
                             }
                         }
@@ -425,19 +506,16 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
                     }
                 }
                 float lv[KB / 8][2];  // log2 of the values' scales
+                if (E4M3) {
+                    const float* sk = reinterpret_cast<const float*>(smem + (base - smem_addr(smem)) + kSK) + kb + 2 * c;
 #pragma unroll
-                for (int i = 0; i < KB / 8; ++i) {
-                    float ks0 = 1.f, ks1 = 1.f;
-                    if (E4M3) {
-                        const float* sk = reinterpret_cast<const float*>(smem + (base - smem_addr(smem)) + kSK) + kb + i * 8 + 2 * c;
-                        const float* sv = sk + WR * KW;
-                        ks0 = sk[0];
-                        ks1 = sk[1];
-                        lv[i][0] = __log2f(sv[0]);
-                        lv[i][1] = __log2f(sv[1]);
+                    for (int i = 0; i < KB / 8; ++i) {
+                        const float2 ks = *reinterpret_cast<const float2*>(sk + i * 8), sv = *reinterpret_cast<const float2*>(sk + WR * KW + i * 8);
+                        lv[i][0] = __log2f(sv.x);
+                        lv[i][1] = __log2f(sv.y);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) s[i][x] *= fac[x >> 1] * ((x & 1) ? ks.y : ks.x);
                     }
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) s[i][x] *= fac[x >> 1] * ((x & 1) ? ks1 : ks0);
                 }
                 // mask, where a key of this step is hidden from some row
                 const int wsrc = wk * WR + kb / KW;
@@ -471,6 +549,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
                         tv[i] = fmaxf(tv[i], __shfl_xor_sync(0xffffffffu, tv[i], 1));
                         tv[i] = fmaxf(tv[i], __shfl_xor_sync(0xffffffffu, tv[i], 2));
                     } else {
+                        tm[i] *= fac[i];
                         tv[i] = tm[i];
                     }
                 }
@@ -497,7 +576,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
                     float e[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const float pr = exp2f(s[i][x] - mz[x >> 1]);
+                        const float pr = E4M3 ? exp2f(s[i][x] - mz[x >> 1]) : exp2f(fmaf(s[i][x], fac[x >> 1], -mz[x >> 1]));
                         l[x >> 1] += pr;
                         // a hidden key's scale may be anything
                         e[x] = !E4M3 ? pr : s[i][x] == -INFINITY ? 0.f : exp2f(s[i][x] + lv[i][x & 1] - vz[x >> 1]);
@@ -515,9 +594,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
                     if constexpr (E4M3) {  // even and odd elements of a chunk become two tiles of eight columns
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            const uint32_t u = __byte_perm(f[x], 0, 0x3120);
-                            v[(x >> 1) * 4 + (x & 1)] = e4m3x2_to_f16x2(u & 0xffffu);
-                            v[(x >> 1) * 4 + 2 + (x & 1)] = e4m3x2_to_f16x2(u >> 16);
+                            e4m3x4_to_f16x4(__byte_perm(f[x], 0, 0x3120), v[(x >> 1) * 4 + (x & 1)], v[(x >> 1) * 4 + 2 + (x & 1)]);
                         }
                     } else {
 #pragma unroll
@@ -598,8 +675,8 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
             }
         }
         __syncthreads();
-        const bool whole = r0 == 0 && r1 == rg.rounds;
-        const int slot = at == began ? 0 : 1;
+        const bool whole = r0 == 0 && v1 == rg.rounds;
+        const int slot = at == began ? 0 : 1;  // a CTA leaves at most two pieces: of the item it begins in and of the one it ends in
         const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * 16 * WR;
         const int chunks = a.D / 8;
         const int tile_base = (item - h * row_tiles) * 16 * WR;
@@ -638,7 +715,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
                 }
             }
         }
-        at += n;
+        at += v1 - v0;
         __syncthreads();  // shared memory is refilled by the next piece
     }
 }
@@ -647,16 +724,19 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
 template <typename T>
 __global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int B, int NK, int rows, int ctas, const float* __restrict__ part_ml,
                                                    const float* __restrict__ part_o) {
-    __shared__ int64_t scratch[8];
+    __shared__ int scratch[8];
+    // Launched while the attention kernel runs (its lengths are no result of that kernel).
     const int b = blockIdx.y, item = blockIdx.x;
     const int G = a.Hq / a.Hkv, M = a.S * G, row_tiles = (M + rows - 1) / rows;
-    const int64_t per = (int64_t)a.Hkv * row_tiles;
-    int64_t before, all;
+    const int per = a.Hkv * row_tiles;
+    int before, all;
     sum_rounds(a, B, NK, b, before, all, scratch);
     const Range rg = seq_range(a, b, NK);
-    all *= per;
-    const int64_t s = before * per + (int64_t)item * rg.rounds, e = s + rg.rounds;
-    const int64_t c0 = ((s + 1) * ctas - 1) / all, c1 = (e * ctas - 1) / all;
+    const Pieces pieces(all * per, ctas);
+    const int s = before * per + item * rg.rounds;
+    const int c0 = pieces.cta_of(s + kLead), c1 = pieces.cta_of(s + rg.rounds - 1);
+    // every CTA waits, so that this kernel's end is the attention kernel's end too
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (c0 == c1) return;
     const int h = item / row_tiles, tile_base = (item - h * row_tiles) * rows;
     const int count = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
@@ -666,10 +746,8 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int B, int 
         if (gr >= M) break;
         float top = -INFINITY, sum = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int64_t c = c0; c <= c1; ++c) {
-            const int64_t begin = c * all / ctas;
-            if (begin == (c + 1) * all / ctas) continue;  // a CTA without work
-            const int64_t part = (c * 2 + (begin >= s ? 0 : 1)) * rows + r;
+        for (int c = c0; c <= c1; ++c) {
+            const int64_t part = ((int64_t)c * 2 + (pieces.begin(c) >= s ? 0 : 1)) * rows + r;
             const float m = part_ml[part * 2], l = part_ml[part * 2 + 1];
             const float mn = fmaxf(top, m);
             const float f0 = top == -INFINITY ? 0.f : exp2f(top - mn), f1 = m == -INFINITY ? 0.f : exp2f(m - mn);
@@ -701,6 +779,21 @@ static void allow_smem_once(K kernel, int bytes, std::atomic<uint64_t>& done) {
     done.fetch_or(bit, std::memory_order_release);
 }
 
+template <typename T>
+static void launch_join(const AttnArgs& a, int64_t B, int64_t items, int NK, int rows, int ctas, const float* part_ml,
+                        const float* part_o, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)items, (unsigned)B);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T>, a, (int)B, NK, rows, ctas, part_ml, part_o));
+}
+
 template <typename T, bool E4M3, int DP, int WR>
 static void launch_rows(const AttnArgs& a, int64_t B, const at::Tensor& q) {
     using Sh = Shape<E4M3, DP>;
@@ -709,15 +802,15 @@ static void launch_rows(const AttnArgs& a, int64_t B, const at::Tensor& q) {
     const int rows = 16 * WR, ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount * (Sh::kSmem > 110000 ? 1 : 2);
     const int G = a.Hq / a.Hkv;
     const int64_t row_tiles = ceil_div((int64_t)a.S * G, rows), items = a.Hkv * row_tiles;
-    ATB_ARG(items < (int64_t(1) << 31) && B <= 65535, "paged_attention: too many query rows or sequences");
+    ATB_ARG(B <= 65535 && B * items * (ceil_div((int64_t)a.W * a.page, Sh::kRound) + 1 + kLead) < (int64_t(1) << 31),
+            "paged_attention: too many sequences, query rows or positions for one call");
     const at::Tensor ws = at::empty({(int64_t)ctas * 2 * rows * (a.Dv + 2)}, q.options().dtype(at::kFloat));
     float* part_o = ws.data_ptr<float>();
     float* part_ml = part_o + (int64_t)ctas * 2 * rows * a.Dv;
     cudaStream_t st = current_stream();
     rows_kernel<T, E4M3, DP, WR><<<ctas, 128, Sh::kSmem, st>>>(a, (int)B, part_ml, part_o);
     ATB_LAUNCH_CHECK();
-    join_kernel<T><<<dim3((unsigned)items, (unsigned)B), 128, 0, st>>>(a, (int)B, Sh::kRound, rows, ctas, part_ml, part_o);
-    ATB_LAUNCH_CHECK();
+    launch_join<T>(a, B, items, Sh::kRound, rows, ctas, part_ml, part_o, st);
 }
 
 template <typename T, bool E4M3, int DP>

@@ -57,6 +57,11 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
     asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}\n" : "=r"(r) : "r"(two));
     return r;
 }
+// four e4m3 values: the low two and the high two
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}\n"
+        : "=r"(lo), "=r"(hi) : "r"(four));
+}
 __device__ __forceinline__ void unpack_e4m3x8(const uint2& u, float (&f)[8]) {
     const uint32_t w[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
 #pragma unroll
