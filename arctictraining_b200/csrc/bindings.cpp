@@ -88,8 +88,9 @@ at::Tensor paged_latent_append(const at::Tensor& q_pe, const at::Tensor& kv_a, c
                                const at::Tensor& cos, const at::Tensor& sin, at::Tensor pages, const at::Tensor& table,
                                const at::Tensor& starts, const c10::optional<at::Tensor>& counts,
                                const c10::optional<at::Tensor>& scale);
-at::Tensor paged_read(const at::Tensor& pages, const at::Tensor& table, const at::Tensor& lengths, int64_t max_length,
-                      const c10::optional<at::Tensor>& scale, at::ScalarType dtype);
+std::tuple<at::Tensor, at::Tensor> paged_read(const at::Tensor& k_pages, const c10::optional<at::Tensor>& v_pages, const at::Tensor& table,
+                                              const at::Tensor& lengths, int64_t max_length, const c10::optional<at::Tensor>& k_scale,
+                                              const c10::optional<at::Tensor>& v_scale, at::ScalarType dtype);
 at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
                            const at::Tensor& starts, const c10::optional<at::Tensor>& counts,
                            const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale, double scale,
@@ -164,8 +165,8 @@ TORCH_LIBRARY(atb200, m) {
           &atb::paged_kv_append);
     m.def("paged_latent_append(Tensor q_pe, Tensor kv_a, Tensor norm_weight, float eps, Tensor cos, Tensor sin, Tensor(a!) pages, "
           "Tensor page_table, Tensor starts, Tensor? counts, Tensor(b!)? page_scale) -> Tensor", &atb::paged_latent_append);
-    m.def("paged_read(Tensor pages, Tensor page_table, Tensor lengths, int max_length, Tensor? page_scale, ScalarType dtype) -> Tensor",
-          &atb::paged_read);
+    m.def("paged_read(Tensor k_pages, Tensor? v_pages, Tensor page_table, Tensor lengths, int max_length, Tensor? k_scale, "
+          "Tensor? v_scale, ScalarType dtype) -> (Tensor, Tensor)", &atb::paged_read);
     m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor starts, Tensor? counts, "
           "Tensor? k_scale, Tensor? v_scale, float scale, int window) -> Tensor", &atb::paged_attention);
     m.def("paged_latent_attention(Tensor q_latent, Tensor q_pe, Tensor pages, Tensor page_table, Tensor starts, Tensor? counts, "

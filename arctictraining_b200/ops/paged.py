@@ -166,13 +166,10 @@ def paged_kv_read(
     op = "paged_kv_read"
     if dtype is None:
         dtype = torch.bfloat16 if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype
-    if _use_kernels(k_pages) and dtype in _HALF and k_pages.dim() == 4 and k_pages.shape[-1] % 16 == 0 and k_pages.shape[-1] > 0:
+    if _use_kernels(k_pages) and dtype in _HALF and k_pages.dim() == 4 and k_pages.shape[-1] % 16 == 0 and 0 < k_pages.shape[-1] <= 2048:
         _count()
-        k = _ext.ops().paged_read(k_pages, page_table, lengths, max_length, k_scale, dtype)
-        if v_pages is None:
-            return k, None
-        _count()
-        return k, _ext.ops().paged_read(v_pages, page_table, lengths, max_length, v_scale, dtype)
+        k, v = _ext.ops().paged_read(k_pages, v_pages, page_table, lengths, max_length, k_scale, v_scale, dtype)
+        return k, None if v_pages is None else v
     _refuse(max_length < 0, f"{op}: max_length must be 0 or more")
     out = []
     for pages, scale in ((k_pages, k_scale), (v_pages, v_scale)):
@@ -180,6 +177,7 @@ def paged_kv_read(
             out.append(None)
             continue
         _check_pages(op, pages, scale, k_pages)
+        _refuse(pages.shape != k_pages.shape or pages.dtype != k_pages.dtype, f"{op}: k_pages and v_pages differ")
         _refuse(scale is None and pages.dtype != dtype, f"{op}: the cache must have the result's type or be e4m3")
         _refuse(page_table.dim() != 2, f"{op}: page_table must be int32 [batch, pages]")
         _check_table(op, page_table, lengths, None, pages, page_table.shape[0])
