@@ -4,6 +4,7 @@
 // Query j of a sequence stands at position p = starts + j and sees the cached positions max(0, p - window + 1) .. p:
 // o = sum_t e^(s_t - m) v_t / sum_t e^(s_t - m), s_t = scale q.k_t, in one pass over the keys with the running maximum m.
 // The latent form has one key row [latent | rotary] for all heads and the latent itself as value.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -59,30 +60,13 @@ struct Pieces {
     }
 };
 
-// Rounds of the sequences before `upto`, and of all: by a CTA of 128 threads.
-__device__ __forceinline__ void sum_rounds(const AttnArgs& a, int B, int NK, int upto, int& before, int& all, int* scratch) {
-    int x = 0, y = 0;
-    for (int b = threadIdx.x; b < B; b += 128) {
-        const int n = seq_range(a, b, NK).rounds;
-        y += n;
-        if (b < upto) x += n;
-    }
-    x = __reduce_add_sync(0xffffffffu, x);
-    y = __reduce_add_sync(0xffffffffu, y);
-    if ((threadIdx.x & 31) == 0) {
-        scratch[threadIdx.x >> 5] = x;
-        scratch[4 + (threadIdx.x >> 5)] = y;
-    }
-    __syncthreads();
-    before = scratch[0] + scratch[1] + scratch[2] + scratch[3];
-    all = scratch[4] + scratch[5] + scratch[6] + scratch[7];
-}
-
-// This CTA's piece [at, to) of the line, the sequence that holds its first round (a sequence has `per` items) and that
-// sequence's first round.
-__device__ __forceinline__ void find_piece(const AttnArgs& a, int B, int NK, int per, int& at, int& to, int& b_out, int& line, int* scratch) {
+// The line's division, and of CTA `cta`'s piece [at, to) the sequence that holds its first round (a sequence has `per` items)
+// and that sequence's first round.
+template <int THREADS>
+__device__ __forceinline__ Pieces find_piece(const AttnArgs& a, int B, int NK, int per, int ctas, int cta, int& at, int& to, int& b_out,
+                                             int& line, int* scratch) {
     // thread i looks at sequences [i n, (i + 1) n)
-    const int n = (B + 127) / 128, b0 = threadIdx.x * n, b1 = min(B, b0 + n);
+    const int n = (B + THREADS - 1) / THREADS, b0 = threadIdx.x * n, b1 = min(B, b0 + n);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int mine = 0;
     for (int b = b0; b < b1; ++b) mine += seq_range(a, b, NK).rounds;
@@ -96,13 +80,13 @@ __device__ __forceinline__ void find_piece(const AttnArgs& a, int B, int NK, int
     __syncthreads();
     int base = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) base += scratch[w];
         all += scratch[w];
     }
-    const Pieces pieces(all * per, gridDim.x);
-    at = pieces.begin(blockIdx.x);
-    to = pieces.begin(blockIdx.x + 1);
+    const Pieces pieces(all * per, ctas);
+    at = pieces.begin(cta);
+    to = pieces.begin(cta + 1);
     int lo = (base + incl - mine) * per;
     if (at < to && at >= lo && at < lo + mine * per) {
         int b = b0;
@@ -112,12 +96,22 @@ __device__ __forceinline__ void find_piece(const AttnArgs& a, int B, int NK, int
             lo += r;
             ++b;
         }
-        scratch[4] = b;
-        scratch[5] = lo;
+        scratch[THREADS / 32] = b;
+        scratch[THREADS / 32 + 1] = lo;
     }
     __syncthreads();
-    b_out = scratch[4];
-    line = scratch[5];
+    b_out = scratch[THREADS / 32];
+    line = scratch[THREADS / 32 + 1];
+    return pieces;
+}
+
+// What the join kernel has to do at the begin of CTA k's piece: nothing, or join the `n` pieces of the item that CTA k - 1
+// began and this CTA goes on with; x: sequence, y: item, z: n, w: the first piece is its CTA's first or second.
+__device__ __forceinline__ int4 join_job(const Pieces& pieces, int cta, int at, int to, int b, int line, const Range& rg) {
+    if (cta == 0 || at >= to) return make_int4(0, 0, 0, 0);
+    const int item = (at - line) / rg.rounds, s = line + item * rg.rounds;
+    if (pieces.cta_of(s + kLead) != cta - 1) return make_int4(0, 0, 0, 0);
+    return make_int4(b, item, pieces.cta_of(s + rg.rounds - 1) - cta + 2, pieces.begin(cta - 1) >= s ? 0 : 1);
 }
 
 // ---- tensor-core pieces -----------------------------------------------------------------------------------------------
@@ -217,7 +211,8 @@ struct Shape {
 };
 
 template <typename T, bool E4M3, int DP, int WR>
-__global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, float* __restrict__ part_ml, float* __restrict__ part_o) {
+__global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __restrict__ part_ml,
+                                                    float* __restrict__ part_o) {
     using Sh = Shape<E4M3, DP>;
     using P = typename std::conditional<E4M3, __half, T>::type;  // type of the matrix instruction
     constexpr int WK = 4 / WR, KW = Sh::kKeys, TK = KW * WR, NK = Sh::kRound, RB = Sh::kRowBytes;
@@ -225,7 +220,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
     constexpr int KB = KW < 32 ? KW : 32;  // keys of one softmax step
     constexpr int kVal = E4M3 ? 8 : 4;     // registers of two 16-byte chunks of 16 values
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int scratch[8];
+    __shared__ int scratch[10];
     __shared__ uint32_t s_valid[4][kStages][2];
     __shared__ float s_ml[4][16][2];
 
@@ -238,10 +233,12 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join kernel may be set up meanwhile
     int b, line, at, to;
-    find_piece(a, B, NK, per, at, to, b, line, scratch);
+    const Pieces pieces = find_piece<128>(a, B, NK, per, gridDim.x, blockIdx.x, at, to, b, line, scratch);
+    Range rg;
+    if (at < to) rg = seq_range(a, b, NK);
+    if (threadIdx.x == 0) jobs[blockIdx.x] = join_job(pieces, blockIdx.x, at, to, b, line, rg);
     if (at >= to) return;
     const int began = at;
-    Range rg = seq_range(a, b, NK);
 
     const uint32_t ring = smem_addr(smem) + wk * WR * kStages * Sh::kStageBytes;
     // of a stage: keys of all warps of the ring, values, key scales, value scales
@@ -720,52 +717,116 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, floa
     }
 }
 
-// Adds the pieces of the items that several CTAs of the attention kernel worked on, in their order along the keys.
-template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int B, int NK, int rows, int ctas, const float* __restrict__ part_ml,
-                                                   const float* __restrict__ part_o) {
-    __shared__ int scratch[8];
-    // Launched while the attention kernel runs (its lengths are no result of that kernel).
-    const int b = blockIdx.y, item = blockIdx.x;
-    const int G = a.Hq / a.Hkv, M = a.S * G, row_tiles = (M + rows - 1) / rows;
-    const int per = a.Hkv * row_tiles;
-    int before, all;
-    sum_rounds(a, B, NK, b, before, all, scratch);
-    const Range rg = seq_range(a, b, NK);
-    const Pieces pieces(all * per, ctas);
-    const int s = before * per + item * rg.rounds;
-    const int c0 = pieces.cta_of(s + kLead), c1 = pieces.cta_of(s + rg.rounds - 1);
-    // every CTA waits, so that this kernel's end is the attention kernel's end too
+// Adds the pieces of an item that several CTAs of the attention kernel worked on, in their order along the keys.  Such an
+// item lies across the begin of some CTA's piece, so there are fewer of them than CTAs: block (k, y) joins rows
+// [per_block y, per_block (y + 1)) of the item that CTA k - 1 began and CTA k goes on with.  With few pieces each warp takes a
+// row of its own, with many the whole block takes one row after the other.  The kernel is launched while the attention kernel
+// runs, and waits for its end before it reads.
+constexpr int kMaxCtas = 1024;
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) join_kernel(const AttnArgs a, int rows, int per_block, const int4* __restrict__ jobs,
+                                                       const float* __restrict__ part_ml, const float* __restrict__ part_o) {
+    __shared__ float weight[kMaxCtas], s_red[2][THREADS / 32];
+    __shared__ float4 s_o[THREADS];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (c0 == c1) return;
+    const int k = blockIdx.x + 1;
+    const int4 job = jobs[k];
+    const int b = job.x, item = job.y, n = job.z, first_slot = job.w;
+    if (n == 0) return;
+    const int G = a.Hq / a.Hkv, M = a.S * G, row_tiles = (M + rows - 1) / rows;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int h = item / row_tiles, tile_base = (item - h * row_tiles) * rows;
     const int count = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
-    const int chunks = a.Dv / 4;
-    for (int u = threadIdx.x; u < rows * chunks; u += 128) {
-        const int r = u / chunks, x = (u - r * chunks) * 4, gr = tile_base + r;
-        if (gr >= M) break;
-        float top = -INFINITY, sum = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = c0; c <= c1; ++c) {
-            const int64_t part = ((int64_t)c * 2 + (pieces.begin(c) >= s ? 0 : 1)) * rows + r;
-            const float m = part_ml[part * 2], l = part_ml[part * 2 + 1];
-            const float mn = fmaxf(top, m);
-            const float f0 = top == -INFINITY ? 0.f : exp2f(top - mn), f1 = m == -INFINITY ? 0.f : exp2f(m - mn);
-            const float4 o = *reinterpret_cast<const float4*>(part_o + part * a.Dv + x);
-            sum = (top == -INFINITY ? sum : sum * f0) + (m == -INFINITY ? l : l * f1);
-            v.x = v.x * f0 + o.x * f1;
-            v.y = v.y * f0 + o.y * f1;
-            v.z = v.z * f0 + o.z * f1;
-            v.w = v.w * f0 + o.w * f1;
-            top = mn;
-        }
+    // place of row r of piece i: the first or the second that its CTA left
+    auto place = [&](int i, int r) { return ((int64_t)(k - 1 + i) * 2 + (i == 0 ? first_slot : 0)) * rows + r; };
+    // a piece without a finite score has seen nothing, or a NaN that its sum holds
+    auto sum_of = [](float m, float l, float w) { return m == -INFINITY ? l : l * w; };
+    auto store = [&](int gr, int col, const float4& v, float sum) {
         const int j = gr / G, hq = h * G + gr - j * G;
         const bool none = j >= count || sum == 0.f;
         const float inv = __fdividef(1.f, sum);
         uint2 res;
         res.x = none ? 0u : pack2<T>(v.x * inv, v.y * inv);
         res.y = none ? 0u : pack2<T>(v.z * inv, v.w * inv);
-        *reinterpret_cast<uint2*>((T*)a.out + (((int64_t)b * a.S + j) * a.Hq + hq) * a.Dv + x) = res;
+        *reinterpret_cast<uint2*>((T*)a.out + (((int64_t)b * a.S + j) * a.Hq + hq) * a.Dv + col) = res;
+    };
+    const int r_first = blockIdx.y * per_block, r_last = min(min(r_first + per_block, rows), M - tile_base);
+    if (n <= 32 && per_block > 1) {
+        for (int r = r_first + warp; r < r_last; r += THREADS / 32) {
+            const float m = lane < n ? part_ml[place(lane, r) * 2] : -INFINITY, l = lane < n ? part_ml[place(lane, r) * 2 + 1] : 0.f;
+            const float top = warp_max(m);
+            const float w = m == -INFINITY ? 0.f : exp2f(m - top);
+            const float sum = warp_sum(sum_of(m, l, w));
+            __syncwarp();
+            weight[warp * 32 + lane] = w;
+            __syncwarp();
+            for (int u = lane; u < a.Dv / 4; u += 32) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                for (int i = 0; i < n; ++i) {
+                    const float4 o = *reinterpret_cast<const float4*>(part_o + place(i, r) * a.Dv + u * 4);
+                    const float wi = weight[warp * 32 + i];
+                    v.x += o.x * wi;
+                    v.y += o.y * wi;
+                    v.z += o.z * wi;
+                    v.w += o.w * wi;
+                }
+                store(tile_base + r, u * 4, v, sum);
+            }
+        }
+        return;
+    }
+    for (int r = r_first; r < r_last; ++r) {
+        float top = -INFINITY, sum = 0.f;
+        for (int i = threadIdx.x; i < n; i += THREADS) top = fmaxf(top, part_ml[place(i, r) * 2]);
+        top = warp_max(top);
+        if (lane == 0) s_red[0][warp] = top;
+        __syncthreads();
+        top = s_red[0][0];
+#pragma unroll
+        for (int w = 1; w < THREADS / 32; ++w) top = fmaxf(top, s_red[0][w]);
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+            const float m = part_ml[place(i, r) * 2], l = part_ml[place(i, r) * 2 + 1];
+            weight[i] = m == -INFINITY ? 0.f : exp2f(m - top);
+            sum += sum_of(m, l, weight[i]);
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) s_red[1][warp] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) sum += s_red[1][w];
+        // four columns a thread; where they are few, several groups of threads take the pieces in turn
+        const int units = a.Dv / 4, groups = THREADS / units;  // at most 128 units of at least 128 threads
+        const int grp = threadIdx.x / units, u = threadIdx.x - grp * units;
+        {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (grp < groups) {
+#pragma unroll 8
+                for (int i = grp; i < n; i += groups) {
+                    const float4 o = *reinterpret_cast<const float4*>(part_o + place(i, r) * a.Dv + u * 4);
+                    const float w = weight[i];
+                    v.x += o.x * w;
+                    v.y += o.y * w;
+                    v.z += o.z * w;
+                    v.w += o.w * w;
+                }
+            }
+            if (groups > 1) {
+                s_o[threadIdx.x] = v;
+                __syncthreads();
+                if (grp == 0)
+                    for (int x = 1; x < groups; ++x) {
+                        const float4 o = s_o[x * units + u];
+                        v.x += o.x;
+                        v.y += o.y;
+                        v.z += o.z;
+                        v.w += o.w;
+                    }
+            }
+            if (grp == 0) store(tile_base + r, u * 4, v, sum);
+        }
+        __syncthreads();
     }
 }
 
@@ -779,19 +840,33 @@ static void allow_smem_once(K kernel, int bytes, std::atomic<uint64_t>& done) {
     done.fetch_or(bit, std::memory_order_release);
 }
 
-template <typename T>
-static void launch_join(const AttnArgs& a, int64_t B, int64_t items, int NK, int rows, int ctas, const float* part_ml,
-                        const float* part_o, cudaStream_t st) {
+// Per CTA of the attention kernel: one join job and up to two pieces of `rows` rows.
+struct Workspace {
+    at::Tensor buf;
+    int4* jobs;
+    float *ml, *o;
+    Workspace(const at::Tensor& like, int ctas, int rows, int Dv) {
+        const int64_t n = (int64_t)ctas * 2 * rows;
+        buf = at::empty({ctas * 4 + n * (Dv + 2)}, like.options().dtype(at::kFloat));
+        jobs = reinterpret_cast<int4*>(buf.data_ptr());
+        o = buf.data_ptr<float>() + ctas * 4;
+        ml = o + n * Dv;
+    }
+};
+
+template <typename T, int THREADS>
+static void launch_join(const AttnArgs& a, int rows, int per_block, int ctas, const Workspace& ws, cudaStream_t st) {
+    if (ctas < 2) return;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)items, (unsigned)B);
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3((unsigned)(ctas - 1), (unsigned)ceil_div(std::min(rows, a.S * (a.Hq / a.Hkv)), per_block));
+    cfg.blockDim = dim3(THREADS);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T>, a, (int)B, NK, rows, ctas, part_ml, part_o));
+    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T, THREADS>, a, rows, per_block, (const int4*)ws.jobs, (const float*)ws.ml, (const float*)ws.o));
 }
 
 template <typename T, bool E4M3, int DP, int WR>
@@ -799,18 +874,17 @@ static void launch_rows(const AttnArgs& a, int64_t B, const at::Tensor& q) {
     using Sh = Shape<E4M3, DP>;
     static std::atomic<uint64_t> done{0};
     allow_smem_once(rows_kernel<T, E4M3, DP, WR>, Sh::kSmem, done);
-    const int rows = 16 * WR, ctas = at::cuda::getCurrentDeviceProperties()->multiProcessorCount * (Sh::kSmem > 110000 ? 1 : 2);
+    const int rows = 16 * WR;
+    const int ctas = std::min(kMaxCtas, at::cuda::getCurrentDeviceProperties()->multiProcessorCount * (Sh::kSmem > 110000 ? 1 : 2));
     const int G = a.Hq / a.Hkv;
     const int64_t row_tiles = ceil_div((int64_t)a.S * G, rows), items = a.Hkv * row_tiles;
-    ATB_ARG(B <= 65535 && B * items * (ceil_div((int64_t)a.W * a.page, Sh::kRound) + 1 + kLead) < (int64_t(1) << 31),
+    ATB_ARG(B * items * (ceil_div((int64_t)a.W * a.page, Sh::kRound) + 1 + kLead) < (int64_t(1) << 31),
             "paged_attention: too many sequences, query rows or positions for one call");
-    const at::Tensor ws = at::empty({(int64_t)ctas * 2 * rows * (a.Dv + 2)}, q.options().dtype(at::kFloat));
-    float* part_o = ws.data_ptr<float>();
-    float* part_ml = part_o + (int64_t)ctas * 2 * rows * a.Dv;
+    const Workspace ws(q, ctas, rows, a.Dv);
     cudaStream_t st = current_stream();
-    rows_kernel<T, E4M3, DP, WR><<<ctas, 128, Sh::kSmem, st>>>(a, (int)B, part_ml, part_o);
+    rows_kernel<T, E4M3, DP, WR><<<ctas, 128, Sh::kSmem, st>>>(a, (int)B, ws.jobs, ws.ml, ws.o);
     ATB_LAUNCH_CHECK();
-    launch_join<T>(a, B, items, Sh::kRound, rows, ctas, part_ml, part_o, st);
+    launch_join<T, 128>(a, rows, 4, ctas, ws, st);
 }
 
 template <typename T, bool E4M3, int DP>
@@ -829,107 +903,499 @@ static void launch_dims(const AttnArgs& a, int64_t B, const at::Tensor& q) {
 }
 
 // ---- latent attention --------------------------------------------------------------------------------------------------
-template <typename T, bool E4M3>
-__device__ __forceinline__ void load8(const void* base, int64_t at, float (&f)[8]) {
-    if (E4M3) unpack_e4m3x8(*reinterpret_cast<const uint2*>((const uint8_t*)base + at), f);
-    else Vec8<T>::unpack(*reinterpret_cast<const uint4*>((const T*)base + at), f);
-}
+// One key row [latent | rotary] for all heads, the latent being its value too: a row of 1152 bytes meets 2 x 16 MT query
+// rows' products, so with 16 heads and one new token the memory still sets the pace.  A CTA of eight warps keeps the
+// weighted values of its query rows in registers, 64 columns a warp, and takes 64 keys at a time.  Scores: the 36 depth
+// steps of 16 are divided over four groups of warps (whose slice of the queries stays in registers) and the keys over two, so
+// every key byte is read from shared memory once; the four partial sums meet in shared memory, where the softmax is taken by
+// all threads.  Weighted values: every warp reads its own 64 columns of the same tile.  Precision is that of the grouped form.
+constexpr int kLatent = 512, kRotary = 64, kJoint = kLatent + kRotary;
 
-// One CTA per (sequence, new token, query head); its warps take keys in turn and are joined at the end.
-template <typename T, bool E4M3>
-__global__ void __launch_bounds__(128) attention_kernel(const AttnArgs a) {
-    constexpr int kMax = 3;  // chunks of 8 elements a lane: D <= 768
-    __shared__ float s_m[4], s_l[4];
-    __shared__ float s_o[4][512];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.x % a.Hq;
-    const int64_t bj = blockIdx.x / a.Hq;
-    const int64_t b = bj / a.S;
-    const int j = (int)(bj - b * a.S);
-    const int kvh = h / (a.Hq / a.Hkv);
-    const int count = a.counts ? min(a.counts[b], a.S) : a.S;
-    const int64_t pos = (int64_t)a.starts[b] + j;
-    int64_t end = min(min(pos + 1, (int64_t)a.starts[b] + count), (int64_t)a.W * a.page);
-    if (j >= count) end = 0;
-    const int64_t first = a.window > 0 ? max((int64_t)0, pos + 1 - a.window) : 0;
-    float q[kMax][8] = {}, o[kMax][8] = {};
-    for (int i = 0; i < kMax; ++i) {
-        const int e = (lane + 32 * i) * 8;
-        if (e < a.D1) Vec8<T>::unpack(*reinterpret_cast<const uint4*>((const T*)a.q + b * a.q_b + j * a.q_s + h * a.q_h + e), q[i]);
-        else if (e < a.D) Vec8<T>::unpack(*reinterpret_cast<const uint4*>((const T*)a.q2 + b * a.q2_b + j * a.q2_s + h * a.q2_h + e - a.D1), q[i]);
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int64_t t = first + warp; t < end; t += 4) {
-        const int w = (int)t / a.page, off = (int)t - w * a.page;
-        const int pid = a.table[b * a.table_stride + w];
-        if (pid < 0 || pid >= a.P) continue;
-        const int64_t row = (int64_t)kvh * a.page + off;
-        float dot = 0.f;
-        for (int i = 0; i < kMax; ++i) {
-            const int e = (lane + 32 * i) * 8;
-            if (e < a.D) {
-                float k[8];
-                load8<T, E4M3>(a.k_pages, pid * a.k_page + row * a.D + e, k);
-                for (int x = 0; x < 8; ++x) dot += q[i][x] * k[x];
+template <bool E4M3, int MT>
+struct LatentShape {
+    static constexpr int kKeys = 64;
+    static constexpr int kRowBytes = kJoint * (E4M3 ? 1 : 2);
+    static constexpr int kStageBytes = kKeys * kRowBytes + (E4M3 ? kKeys * 4 : 0);
+    static constexpr int kRing = E4M3 ? 4 : 2;
+    static constexpr int kScoreRow = 72;  // floats; 64 keys, spread over the banks
+    static constexpr int kScores = kRing * kStageBytes;
+    static constexpr int kProbs = kScores + 4 * 16 * MT * kScoreRow * 4;
+    static constexpr int kSmem = kProbs + 16 * MT * 128;
+};
+
+template <typename T, bool E4M3, int MT>
+__global__ void __launch_bounds__(256) latent_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __restrict__ part_ml,
+                                                    float* __restrict__ part_o) {
+    using Sh = LatentShape<E4M3, MT>;
+    using P = typename std::conditional<E4M3, __half, T>::type;
+    constexpr int NK = Sh::kKeys, RB = Sh::kRowBytes, CPR = RB / 16, kRing = Sh::kRing, kRows = 16 * MT;
+    constexpr int kSteps = 9;            // depth steps of a warp
+    constexpr int kVal = E4M3 ? 8 : 4;   // registers of two 16-byte chunks of 16 values
+    constexpr int kVChunks = 64 * (E4M3 ? 1 : 2) / 16;  // a warp's chunks of a value row
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int scratch[10];
+    __shared__ uint32_t s_valid[kRing][2];
+    __shared__ float s_grow[kRows], s_fac[kRows], s_m[kRows], s_l[kRows];
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int dg = warp & 3, kh = warp >> 2;
+    const int H = a.Hq, M = a.S * H, per = (M + kRows - 1) / kRows;
+
+    int b, line, at, to;
+    const Pieces pieces = find_piece<256>(a, B, NK, per, gridDim.x, blockIdx.x, at, to, b, line, scratch);
+    Range rg;
+    if (at < to) rg = seq_range(a, b, NK);
+    if (threadIdx.x == 0) jobs[blockIdx.x] = join_job(pieces, blockIdx.x, at, to, b, line, rg);
+    if (at >= to) return;
+    const int began = at;
+    const uint32_t ring = smem_addr(smem);
+    float* scores = reinterpret_cast<float*>(smem + Sh::kScores);
+    const uint32_t probs = smem_addr(smem) + Sh::kProbs;
+    // place of a 16-byte chunk in a row: exchanged by the row's low bits so that eight rows meet different banks
+    auto chunk_at = [](int key, int ch) { return (E4M3 ? ch ^ ((key >> 1) & 3) : ch ^ (key & 7)) * 16; };
+
+    while (at < to) {
+        while (at >= line + rg.rounds * per) {
+            line += rg.rounds * per;
+            ++b;
+            rg = seq_range(a, b, NK);
+        }
+        const int item = (at - line) / rg.rounds;
+        const int v0 = at - line - item * rg.rounds, v1 = min(rg.rounds, v0 + (to - at));
+        const int r0 = max(0, v0 - kLead), r1 = v1 - kLead;
+        if (r1 <= r0) {
+            at += v1 - v0;
+            continue;
+        }
+        const int n = r1 - r0, tile_base = item * kRows;
+        const int* table = a.table + b * a.table_stride;
+
+        // copies of tile t: four threads a key
+        const int my_key = tid >> 2, my_part = tid & 3;
+        int look_w, look_off, look_key = rg.first + r0 * NK + my_key, pid_next;
+        look_w = look_key / a.page;
+        look_off = look_key - look_w * a.page;
+        const int step_w = NK / a.page, step_off = NK - step_w * a.page;
+        auto look_up = [&](int t) {
+            pid_next = -1;
+            if (t < n && look_key < rg.total) pid_next = table[look_w];
+        };
+        auto issue = [&](int t) {
+            if (t < n) {
+                const int st = t % kRing;
+                const uint32_t base = ring + st * Sh::kStageBytes + my_key * RB;
+                const bool ok = pid_next >= 0 && pid_next < a.P;
+                const uint8_t* src = (const uint8_t*)a.k_pages + (ok ? pid_next * a.k_page + (int64_t)look_off * a.D : 0) * (E4M3 ? 1 : 2);
+                const int lat = a.D1 * (E4M3 ? 1 : 2), all = a.D * (E4M3 ? 1 : 2);
+                constexpr int kLatChunks = kLatent * (E4M3 ? 1 : 2) / 16;
+#pragma unroll
+                for (int i = 0; i < CPR / 4; ++i) {
+                    const int ch = i * 4 + my_part;
+                    // narrower latents leave zeros between themselves and the rotary part
+                    const int byte = ch < kLatChunks ? ch * 16 : lat + (ch - kLatChunks) * 16;
+                    const bool full = ok && (ch < kLatChunks ? byte < lat : byte < all);
+                    copy16(base + chunk_at(my_key, ch), full ? src + byte : (const uint8_t*)a.k_pages, full);
+                }
+                if (E4M3 && my_part == 0)
+                    copy4(ring + st * Sh::kStageBytes + NK * RB + my_key * 4, a.k_scale + (ok ? pid_next * a.ks_page + look_off : 0), ok);
+                // eight keys a warp: their bits, gathered from the first lane of each
+                const uint32_t bits = __ballot_sync(0xffffffffu, ok);
+                if (lane == 0) {
+                    uint32_t eight = 0;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) eight |= ((bits >> (4 * k)) & 1u) << k;
+                    reinterpret_cast<uint8_t*>(s_valid[st])[warp] = (uint8_t)eight;
+                }
+                look_key += NK;
+                look_w += step_w;
+                look_off += step_off;
+                if (look_off >= a.page) {
+                    look_off -= a.page;
+                    ++look_w;
+                }
+            }
+            copies_commit();
+        };
+
+        look_up(0);
+#pragma unroll
+        for (int t = 0; t < kRing - 1; ++t) {
+            issue(t);
+            look_up(t + 1);
+        }
+
+        // this warp's depth slice of the queries
+        auto q_src = [&](int r, int col) -> const T* {  // element `col` of the joint row of query row r, or null
+            const int gr = tile_base + r;
+            if (gr >= M) return nullptr;
+            const int j = gr / H, h = gr - j * H;
+            if (col < kLatent) return col < a.D1 ? (const T*)a.q + b * a.q_b + j * a.q_s + h * a.q_h + col : nullptr;
+            return col - kLatent < a.D - a.D1 ? (const T*)a.q2 + b * a.q2_b + j * a.q2_s + h * a.q2_h + col - kLatent : nullptr;
+        };
+        // |scale| log2 e and, for bf16 queries against an 8-bit cache, the inverse of the row's power of two (see above)
+        float up[MT][2];
+        if (E4M3 && std::is_same<T, bf16>::value) {
+            for (int r = warp; r < kRows; r += 8) {
+                float m = 0.f;
+                for (int col = lane * 2; col < kJoint; col += 64) {
+                    const T* src = q_src(r, col);
+                    if (src) {
+                        const float2 x = unpack2<T>(*reinterpret_cast<const uint32_t*>(src));
+                        m = fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y)));
+                    }
+                }
+                m = warp_max(m);
+                const int e = (__float_as_uint(m) >> 23) & 255;
+                if (lane == 0) s_fac[r] = __uint_as_float((uint32_t)(e == 0 || e == 255 ? 127 : min(268 - e, 253)) << 23);
+            }
+            __syncthreads();
+        }
+        uint32_t q[MT][kSteps][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = mt * 16 + g + 8 * i;
+                if (E4M3 && std::is_same<T, bf16>::value) up[mt][i] = s_fac[r];
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    const int col = (dg * kSteps + k) * 16;
+                    uint32_t x = 0, y = 0;
+                    if (E4M3) {
+                        const T* src = q_src(r, col);
+                        if (src) {
+                            const uint2 u = *reinterpret_cast<const uint2*>(src + 4 * c);
+                            x = u.x;
+                            y = u.y;
+                        }
+                    } else {
+                        const T* src = q_src(r, col);
+                        if (src) {
+                            x = *reinterpret_cast<const uint32_t*>(src + 2 * c);
+                            y = *reinterpret_cast<const uint32_t*>(src + 8 + 2 * c);
+                        }
+                    }
+                    if (a.scale < 0.f) {
+                        x ^= 0x80008000u;
+                        y ^= 0x80008000u;
+                    }
+                    if (E4M3 && std::is_same<T, bf16>::value) {
+                        const float2 fx = unpack2<T>(x), fy = unpack2<T>(y);
+                        x = pack2<__half>(fx.x * up[mt][i], fx.y * up[mt][i]);
+                        y = pack2<__half>(fy.x * up[mt][i], fy.y * up[mt][i]);
+                    }
+                    q[mt][k][i] = x;
+                    q[mt][k][i + 2] = y;
+                }
+            }
+
+        // softmax: kLanes threads a row, kCols keys each
+        constexpr int kLanes = 256 / kRows, kCols = NK / kLanes;
+        const int srow = tid / kLanes, scol = (tid % kLanes) * kCols;
+        const int sj = min(tile_base + srow, M - 1) / H;
+        const int hi = (int)min((int64_t)rg.start + sj, (int64_t)rg.total - 1);
+        float fac = fmaxf(fabsf(a.scale), 1e-30f) * kLog2e;
+        if (E4M3 && std::is_same<T, bf16>::value) fac *= __uint_as_float((254u << 23) - __float_as_uint(s_fac[srow]));
+        float m = -INFINITY, mv = -INFINITY, l = 0.f;
+        float o[MT][8][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[mt][i][x] = 0.f;
+
+        for (int t = 0; t < n; ++t) {
+            copies_wait<kRing - 2>();
+            __syncthreads();  // tile t is here; every warp is done with tile t - 1
+            issue(t + kRing - 1);
+            look_up(t + kRing);
+            const int st = t % kRing;
+            const uint32_t base = ring + st * Sh::kStageBytes;
+            const int first = rg.first + (r0 + t) * NK;
+            // scores of this warp's 32 keys and depth slice
+            {
+                float s[MT][4][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) s[mt][i][x] = 0.f;
+                const int r = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1;
+#pragma unroll
+                for (int kp = 0; kp < 2; ++kp) {
+                    const int key = kh * 32 + kp * 16 + r;
+                    const uint32_t krow = base + key * RB;
+                    if (E4M3) {
+#pragma unroll
+                        for (int k = 0; k < kSteps; k += 2) {
+                            uint32_t f[4];
+                            // the ninth step has no partner: its second half is read again and not used
+                            const int ch = dg * kSteps + min(k + half, kSteps - 1);
+                            ldsm4(f, krow + chunk_at(key, ch));
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                if (k + (x & 1) >= kSteps) continue;
+                                uint32_t b0, b1;
+                                e4m3x4_to_f16x4(f[x], b0, b1);
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) mma<P>(s[mt][2 * kp + (x >> 1)], q[mt][k + (x & 1)], b0, b1);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < kSteps; ++k) {
+                            uint32_t f[4];
+                            ldsm4(f, krow + chunk_at(key, 2 * (dg * kSteps + k) + half));
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                mma<P>(s[mt][2 * kp], q[mt][k], f[0], f[1]);
+                                mma<P>(s[mt][2 * kp + 1], q[mt][k], f[2], f[3]);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float* dst = scores + (dg * kRows + mt * 16 + g) * Sh::kScoreRow + kh * 32 + i * 8 + 2 * c;
+                        *reinterpret_cast<float2*>(dst) = make_float2(s[mt][i][0], s[mt][i][1]);
+                        *reinterpret_cast<float2*>(dst + 8 * Sh::kScoreRow) = make_float2(s[mt][i][2], s[mt][i][3]);
+                    }
+            }
+            __syncthreads();
+            // softmax of the tile
+            {
+                float x[kCols], lv[kCols];
+#pragma unroll
+                for (int i = 0; i < kCols; i += 4) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        const float4 y = *reinterpret_cast<const float4*>(scores + (d * kRows + srow) * Sh::kScoreRow + scol + i);
+                        v.x += y.x;
+                        v.y += y.y;
+                        v.z += y.z;
+                        v.w += y.w;
+                    }
+                    x[i] = v.x * fac;
+                    x[i + 1] = v.y * fac;
+                    x[i + 2] = v.z * fac;
+                    x[i + 3] = v.w * fac;
+                }
+                if (E4M3) {
+                    const float* sc = reinterpret_cast<const float*>(smem + st * Sh::kStageBytes + NK * RB) + scol;
+#pragma unroll
+                    for (int i = 0; i < kCols; ++i) {
+                        const float y = sc[i];
+                        x[i] *= y;
+                        lv[i] = __log2f(y);
+                    }
+                }
+                const uint32_t valid = s_valid[st][scol >> 5] >> (scol & 31);
+                float tm = -INFINITY, tv = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) {
+                    if (first + scol + i > hi || !((valid >> i) & 1)) x[i] = -INFINITY;
+                    tm = fmaxf(tm, x[i]);
+                    if (E4M3) tv = fmaxf(tv, x[i] + lv[i]);
+                }
+#pragma unroll
+                for (int d = 1; d < kLanes; d <<= 1) {
+                    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, d));
+                    if (E4M3) tv = fmaxf(tv, __shfl_xor_sync(0xffffffffu, tv, d));
+                }
+                if (!E4M3) tv = tm;
+                const float mn = fmaxf(m, tm), vn = fmaxf(mv, tv);
+                l *= m == -INFINITY ? 0.f : exp2f(m - mn);
+                if (tid % kLanes == 0) s_grow[srow] = mv == -INFINITY ? 0.f : exp2f(mv - vn);
+                m = mn;
+                mv = vn;
+                const float mz = m == -INFINITY ? 0.f : m, vz = mv == -INFINITY ? 0.f : mv;
+                uint32_t w[kCols / 2];
+#pragma unroll
+                for (int i = 0; i < kCols; i += 2) {
+                    float e[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float pr = exp2f(x[i + k] - mz);
+                        l += pr;
+                        e[k] = !E4M3 ? pr : x[i + k] == -INFINITY ? 0.f : exp2f(x[i + k] + lv[i + k] - vz);
+                    }
+                    w[i / 2] = pack2<P>(e[0], e[1]);
+                }
+                uint8_t* dst = smem + Sh::kProbs + srow * 128;
+                const int ch = scol / 8;
+                if (kCols == 4) *reinterpret_cast<uint2*>(dst + ((ch ^ (srow & 7)) * 16) + (scol & 4) * 2) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint4*>(dst + ((ch ^ (srow & 7)) * 16)) = make_uint4(w[0], w[1], w[kCols / 2 - 2], w[kCols / 2 - 1]);
+            }
+            __syncthreads();
+            // weighted values of this warp's 64 columns
+            {
+                bool grew = false;
+                float f[MT][2];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        f[mt][i] = s_grow[mt * 16 + g + 8 * i];
+                        grew = grew || f[mt][i] != 1.f;
+                    }
+                if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) o[mt][i][x] *= f[mt][x >> 1];
+                }
+                auto load_probs = [&](int mt, int kp, uint32_t (&p)[4]) {
+                    const int r = mt * 16 + (lane & 15);
+                    ldsm4(p, probs + r * 128 + (((kp * 2 + (lane >> 4)) ^ (r & 7)) * 16));
+                };
+                auto load_values = [&](int kp, int k, uint32_t (&v)[kVal]) {
+                    const int key = kp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+                    uint32_t x[4];
+                    ldsm4_t(x, base + key * RB + chunk_at(key, warp * kVChunks + k + (lane >> 4)));
+                    if constexpr (E4M3) {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+                            e4m3x4_to_f16x4(__byte_perm(x[y], 0, 0x3120), v[(y >> 1) * 4 + (y & 1)], v[(y >> 1) * 4 + 2 + (y & 1)]);
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) v[y] = x[y];
+                    }
+                };
+                const bool hidden = a.S > 1 && first + NK - 1 > rg.start;
+                if (hidden && values_not_finite<P, kVal, 4, kVChunks>(load_values)) {
+                    // see the grouped form: each new token's rows get a product without the keys hidden from them
+                    const int last = min(tile_base + kRows - 1, M - 1) / H;
+                    for (int j = tile_base / H; j <= last; ++j) {
+                        const int hj = (int)min((int64_t)rg.start + j, (int64_t)rg.total - 1);
+#pragma unroll 1
+                        for (int kp = 0; kp < 4; ++kp) {
+                            uint32_t keep[2], p[MT][4];
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const int pos = first + kp * 16 + 8 * x + 2 * c;
+                                keep[x] = (pos <= hj ? 0xffffu : 0u) | (pos + 1 <= hj ? 0xffff0000u : 0u);
+                            }
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) load_probs(mt, kp, p[mt]);
+#pragma unroll
+                            for (int k = 0; k < kVChunks; k += 2) {
+                                uint32_t v[kVal];
+                                load_values(kp, k, v);
+#pragma unroll
+                                for (int x = 0; x < kVal / 2; ++x)
+#pragma unroll
+                                    for (int mt = 0; mt < MT; ++mt) {
+                                        float add[4] = {0.f, 0.f, 0.f, 0.f};
+                                        mma<P>(add, p[mt], v[2 * x] & keep[0], v[2 * x + 1] & keep[1]);
+#pragma unroll
+                                        for (int y = 0; y < 4; ++y)
+                                            if (min(tile_base + mt * 16 + g + 8 * (y >> 1), M - 1) / H == j) o[mt][k * (kVal / 4) + x][y] += add[y];
+                                    }
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int kp = 0; kp < 4; ++kp) {
+                        uint32_t p[MT][4];
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) load_probs(mt, kp, p[mt]);
+#pragma unroll
+                        for (int k = 0; k < kVChunks; k += 2) {
+                            uint32_t v[kVal];
+                            load_values(kp, k, v);
+#pragma unroll
+                            for (int x = 0; x < kVal / 2; ++x)
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) mma<P>(o[mt][k * (kVal / 4) + x], p[mt], v[2 * x], v[2 * x + 1]);
+                        }
+                    }
+                }
             }
         }
-        dot = warp_sum(dot) * a.scale;
-        if (E4M3) dot *= a.k_scale[pid * a.ks_page + row];
-        const float mn = max_nan(m, dot);
-        const float c = m == -INFINITY ? 0.f : __expf(m - mn);
-        const float p = mn == -INFINITY ? 0.f : __expf(dot - mn);
-        m = mn;
-        l = l * c + p;
-        const float pv = E4M3 ? p * a.v_scale[pid * a.vs_page + row] : p;
-        for (int i = 0; i < kMax; ++i) {
-            const int e = (lane + 32 * i) * 8;
-            if (e < a.Dv) {
-                float v[8];
-                load8<T, E4M3>(a.v_pages, pid * a.v_page + row * a.D + e, v);
-                for (int x = 0; x < 8; ++x) o[i][x] = o[i][x] * c + pv * v[x];
+        copies_wait<0>();
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        __syncthreads();  // the last tile's s_grow has been read
+        if (tid % kLanes == 0) {
+            s_m[srow] = m;
+            s_l[srow] = l;
+            s_grow[srow] = !E4M3 ? 1.f : mv == -INFINITY ? 0.f : exp2f(mv - m);  // weighted values are in units of 2^mv
+        }
+        __syncthreads();
+        const bool whole = r0 == 0 && v1 == rg.rounds;
+        const int slot = at == began ? 0 : 1;
+        const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * kRows;
+        const int count = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = mt * 16 + g + 8 * i, gr = tile_base + r;
+                if (gr >= M) continue;
+                const float f = s_grow[r], sum = s_l[r];
+                const bool none = gr / H >= count || sum == 0.f;
+                const float inv = whole ? __fdividef(f, sum) : f;
+                T* out = (T*)a.out + (((int64_t)b * a.S * H) + gr) * a.Dv;
+                float* dst = part_o + (part + r) * a.Dv;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // 16 columns: two tiles of eight, or (8-bit) of even and of odd columns
+                    const int col = warp * 64 + k * 16;
+                    if (col >= a.Dv) continue;
+                    float e[4] = {o[mt][2 * k][2 * i] * inv, o[mt][2 * k][2 * i + 1] * inv, o[mt][2 * k + 1][2 * i] * inv,
+                                  o[mt][2 * k + 1][2 * i + 1] * inv};
+                    const int at0 = E4M3 ? col + 4 * c : col + 2 * c, at1 = E4M3 ? at0 + 2 : at0 + 8;
+                    if (E4M3) {
+                        const float x = e[1];
+                        e[1] = e[2];
+                        e[2] = x;
+                    }
+                    if (whole) {
+                        *reinterpret_cast<uint32_t*>(out + at0) = none ? 0u : pack2<T>(e[0], e[1]);
+                        *reinterpret_cast<uint32_t*>(out + at1) = none ? 0u : pack2<T>(e[2], e[3]);
+                    } else {
+                        *reinterpret_cast<float2*>(dst + at0) = make_float2(e[0], e[1]);
+                        *reinterpret_cast<float2*>(dst + at1) = make_float2(e[2], e[3]);
+                    }
+                }
+                if (!whole && warp == 0 && c == 0) {
+                    part_ml[(part + r) * 2] = s_m[r];
+                    part_ml[(part + r) * 2 + 1] = sum;
+                }
             }
-        }
-    }
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
-    for (int i = 0; i < kMax; ++i) {
-        const int e = (lane + 32 * i) * 8;
-        if (e < a.Dv)
-            for (int x = 0; x < 8; ++x) s_o[warp][e + x] = o[i][x];
-    }
-    __syncthreads();
-    float top = -INFINITY;
-    for (int w = 0; w < 4; ++w) top = max_nan(top, s_m[w]);
-    float total = 0.f, f[4];
-    for (int w = 0; w < 4; ++w) {
-        f[w] = s_m[w] == -INFINITY ? 0.f : __expf(s_m[w] - top);
-        total += f[w] * s_l[w];
-    }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    for (int e = threadIdx.x * 8; e < a.Dv; e += 128 * 8) {
-        float r[8];
-        for (int x = 0; x < 8; ++x) {
-            r[x] = 0.f;
-            for (int w = 0; w < 4; ++w) r[x] += f[w] == 0.f ? 0.f : f[w] * s_o[w][e + x];
-            r[x] *= inv;
-        }
-        *reinterpret_cast<uint4*>((T*)a.out + (bj * a.Hq + h) * a.Dv + e) = Vec8<T>::pack(r);
+        at += v1 - v0;
+        __syncthreads();
     }
 }
 
-static void launch_attention(const at::Tensor& q, bool f8, const AttnArgs& a, int64_t B) {
+template <typename T, bool E4M3, int MT>
+static void launch_latent_rows(const AttnArgs& a, int64_t B, const at::Tensor& q) {
+    using Sh = LatentShape<E4M3, MT>;
+    static std::atomic<uint64_t> done{0};
+    allow_smem_once(latent_kernel<T, E4M3, MT>, Sh::kSmem, done);
+    const int rows = 16 * MT, ctas = std::min(kMaxCtas, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+    const int64_t items = ceil_div((int64_t)a.S * a.Hq, rows);
+    ATB_ARG(B * items * (ceil_div((int64_t)a.W * a.page, Sh::kKeys) + 1 + kLead) < (int64_t(1) << 31),
+            "paged_latent_attention: too many sequences, query rows or positions for one call");
+    const Workspace ws(q, ctas, rows, a.Dv);
     cudaStream_t st = current_stream();
-    const dim3 grid((unsigned)(B * a.S * a.Hq));
-    if (q.scalar_type() == at::kBFloat16) {
-        if (f8) attention_kernel<bf16, true><<<grid, 128, 0, st>>>(a);
-        else attention_kernel<bf16, false><<<grid, 128, 0, st>>>(a);
-    } else {
-        if (f8) attention_kernel<__half, true><<<grid, 128, 0, st>>>(a);
-        else attention_kernel<__half, false><<<grid, 128, 0, st>>>(a);
-    }
+    latent_kernel<T, E4M3, MT><<<ctas, 256, Sh::kSmem, st>>>(a, (int)B, ws.jobs, ws.ml, ws.o);
     ATB_LAUNCH_CHECK();
+    launch_join<T, 256>(a, rows, 1, ctas, ws, st);
+}
+
+template <typename T, bool E4M3>
+static void launch_latent(const AttnArgs& a, int64_t B, const at::Tensor& q) {
+    if (a.S * a.Hq <= 16) launch_latent_rows<T, E4M3, 1>(a, B, q);
+    else launch_latent_rows<T, E4M3, 2>(a, B, q);
 }
 
 static bool half_type(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
@@ -1016,7 +1482,9 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& q_pe, c
     a.table_stride = table.stride(0);
     a.S = (int)S; a.Hq = (int)H; a.Hkv = 1; a.D = (int)(R + rope); a.D1 = a.Dv = (int)R; a.P = (int)pages.size(0);
     a.W = (int)table.size(1); a.page = (int)pages.size(2); a.window = 0; a.scale = (float)scale;
-    launch_attention(q, is_e4m3(pages), a, B);
+    const bool f8 = is_e4m3(pages);
+    if (q.scalar_type() == at::kBFloat16) f8 ? launch_latent<bf16, true>(a, B, q) : launch_latent<bf16, false>(a, B, q);
+    else f8 ? launch_latent<__half, true>(a, B, q) : launch_latent<__half, false>(a, B, q);
     return out;
 }
 
