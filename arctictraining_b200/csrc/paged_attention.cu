@@ -717,116 +717,123 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, int4
     }
 }
 
-// Adds the pieces of an item that several CTAs of the attention kernel worked on, in their order along the keys.  Such an
-// item lies across the begin of some CTA's piece, so there are fewer of them than CTAs: block (k, y) joins rows
-// [per_block y, per_block (y + 1)) of the item that CTA k - 1 began and CTA k goes on with.  With few pieces each warp takes a
-// row of its own, with many the whole block takes one row after the other.  The kernel is launched while the attention kernel
-// runs, and waits for its end before it reads.
+// Adds the pieces of an item that several CTAs of the attention kernel worked on, in their order along the keys.  Such an item
+// lies across the begin of some CTA's piece; the attention kernel left a job there.  Every block gathers the jobs (their order
+// does not matter) and the blocks share out (job, query row, 128 columns): a warp each where the items have few pieces, a block
+// each, its warps taking pieces in turn, where some item has many.  The kernel is launched while the attention kernel runs, and
+// waits for its end before it reads.
 constexpr int kMaxCtas = 1024;
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS) join_kernel(const AttnArgs a, int rows, int per_block, const int4* __restrict__ jobs,
-                                                       const float* __restrict__ part_ml, const float* __restrict__ part_o) {
-    __shared__ float weight[kMaxCtas], s_red[2][THREADS / 32];
-    __shared__ float4 s_o[THREADS];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int k = blockIdx.x + 1;
-    const int4 job = jobs[k];
-    const int b = job.x, item = job.y, n = job.z, first_slot = job.w;
-    if (n == 0) return;
-    const int G = a.Hq / a.Hkv, M = a.S * G, row_tiles = (M + rows - 1) / rows;
+template <typename T>
+__global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int rows, int ctas, const int4* __restrict__ jobs,
+                                                   const float* __restrict__ part_ml, const float* __restrict__ part_o) {
+    __shared__ int4 s_jobs[kMaxCtas];
+    __shared__ int s_first[kMaxCtas], s_count, s_most;
+    __shared__ float2 s_ml[kMaxCtas];
+    __shared__ float s_red[2][4];
+    __shared__ float4 s_o[128];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int h = item / row_tiles, tile_base = (item - h * row_tiles) * rows;
-    const int count = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
-    // place of row r of piece i: the first or the second that its CTA left
-    auto place = [&](int i, int r) { return ((int64_t)(k - 1 + i) * 2 + (i == 0 ? first_slot : 0)) * rows + r; };
-    // a piece without a finite score has seen nothing, or a NaN that its sum holds
-    auto sum_of = [](float m, float l, float w) { return m == -INFINITY ? l : l * w; };
-    auto store = [&](int gr, int col, const float4& v, float sum) {
-        const int j = gr / G, hq = h * G + gr - j * G;
-        const bool none = j >= count || sum == 0.f;
-        const float inv = __fdividef(1.f, sum);
-        uint2 res;
-        res.x = none ? 0u : pack2<T>(v.x * inv, v.y * inv);
-        res.y = none ? 0u : pack2<T>(v.z * inv, v.w * inv);
-        *reinterpret_cast<uint2*>((T*)a.out + (((int64_t)b * a.S + j) * a.Hq + hq) * a.Dv + col) = res;
-    };
-    const int r_first = blockIdx.y * per_block, r_last = min(min(r_first + per_block, rows), M - tile_base);
-    if (n <= 32 && per_block > 1) {
-        for (int r = r_first + warp; r < r_last; r += THREADS / 32) {
-            const float m = lane < n ? part_ml[place(lane, r) * 2] : -INFINITY, l = lane < n ? part_ml[place(lane, r) * 2 + 1] : 0.f;
-            const float top = warp_max(m);
-            const float w = m == -INFINITY ? 0.f : exp2f(m - top);
-            const float sum = warp_sum(sum_of(m, l, w));
-            __syncwarp();
-            weight[warp * 32 + lane] = w;
-            __syncwarp();
-            for (int u = lane; u < a.Dv / 4; u += 32) {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                for (int i = 0; i < n; ++i) {
-                    const float4 o = *reinterpret_cast<const float4*>(part_o + place(i, r) * a.Dv + u * 4);
-                    const float wi = weight[warp * 32 + i];
-                    v.x += o.x * wi;
-                    v.y += o.y * wi;
-                    v.z += o.z * wi;
-                    v.w += o.w * wi;
-                }
-                store(tile_base + r, u * 4, v, sum);
-            }
-        }
-        return;
+    const int G = a.Hq / a.Hkv, M = a.S * G, row_tiles = (M + rows - 1) / rows;
+    if (threadIdx.x == 0) s_count = s_most = 0;
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int4 mine[kMaxCtas / 128];
+#pragma unroll
+    for (int x = 0; x < kMaxCtas / 128; ++x) {
+        const int k = threadIdx.x + 128 * x;
+        mine[x] = k < ctas ? jobs[k] : make_int4(0, 0, 0, 0);
     }
-    for (int r = r_first; r < r_last; ++r) {
-        float top = -INFINITY, sum = 0.f;
-        for (int i = threadIdx.x; i < n; i += THREADS) top = fmaxf(top, part_ml[place(i, r) * 2]);
-        top = warp_max(top);
-        if (lane == 0) s_red[0][warp] = top;
-        __syncthreads();
-        top = s_red[0][0];
 #pragma unroll
-        for (int w = 1; w < THREADS / 32; ++w) top = fmaxf(top, s_red[0][w]);
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-            const float m = part_ml[place(i, r) * 2], l = part_ml[place(i, r) * 2 + 1];
-            weight[i] = m == -INFINITY ? 0.f : exp2f(m - top);
-            sum += sum_of(m, l, weight[i]);
+    for (int x = 0; x < kMaxCtas / 128; ++x)
+        if (mine[x].z > 0) {
+            const int at = atomicAdd(&s_count, 1);
+            s_jobs[at] = mine[x];
+            s_first[at] = threadIdx.x + 128 * x - 1;
+            atomicMax(&s_most, mine[x].z);
         }
-        sum = warp_sum(sum);
-        if (lane == 0) s_red[1][warp] = sum;
-        __syncthreads();
-        sum = 0.f;
+    __syncthreads();
+    const int used = row_tiles > 1 ? rows : M, slices = (a.Dv / 4 + 31) / 32;
+    const int total = s_count * used * slices;
+    const bool wide = s_most > 8;  // a block for each unit
+    for (int u = wide ? blockIdx.x : blockIdx.x * 4 + warp; u < total; u += wide ? gridDim.x : gridDim.x * 4) {
+        const int col = (u % slices) * 128 + lane * 4, rest = u / slices;
+        const int r = rest % used, jb = rest / used;
+        const int4 job = s_jobs[jb];
+        const int b = job.x, n = job.z, cta = s_first[jb], h = job.y / row_tiles, gr = (job.y - h * row_tiles) * rows + r;
+        if (gr >= M) continue;
+        // place of piece i: the first or the second that its CTA left
+        auto place = [&](int i) { return ((int64_t)(cta + i) * 2 + (i == 0 ? job.w : 0)) * rows + r; };
+        // a piece without a finite score has seen nothing, or a NaN that its sum holds
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float top = -INFINITY, sum = 0.f;
+        if (!wide) {
+            const float2 ml = lane < n ? *reinterpret_cast<const float2*>(part_ml + place(lane) * 2) : make_float2(-INFINITY, 0.f);
+            float4 o[8];
 #pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) sum += s_red[1][w];
-        // four columns a thread; where they are few, several groups of threads take the pieces in turn
-        const int units = a.Dv / 4, groups = THREADS / units;  // at most 128 units of at least 128 threads
-        const int grp = threadIdx.x / units, u = threadIdx.x - grp * units;
-        {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (grp < groups) {
+            for (int i = 0; i < 8; ++i)
+                o[i] = i < n && col < a.Dv ? *reinterpret_cast<const float4*>(part_o + place(i) * a.Dv + col) : v;
+            top = warp_max(ml.x);
+            const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+            sum = warp_sum(ml.x == -INFINITY ? ml.y : ml.y * w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float wi = __shfl_sync(0xffffffffu, w, i);
+                v.x += o[i].x * wi;
+                v.y += o[i].y * wi;
+                v.z += o[i].z * wi;
+                v.w += o[i].w * wi;
+            }
+        } else {
+            __syncthreads();  // the unit before is done with shared memory
+            for (int i = threadIdx.x; i < n; i += 128) {
+                s_ml[i] = *reinterpret_cast<const float2*>(part_ml + place(i) * 2);
+                top = fmaxf(top, s_ml[i].x);
+            }
+            top = warp_max(top);
+            if (lane == 0) s_red[0][warp] = top;
+            __syncthreads();
+            top = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+            for (int i = threadIdx.x; i < n; i += 128) {
+                const float m = s_ml[i].x, l = s_ml[i].y, w = m == -INFINITY ? 0.f : exp2f(m - top);
+                s_ml[i].x = w;
+                sum += m == -INFINITY ? l : l * w;
+            }
+            sum = warp_sum(sum);
+            if (lane == 0) s_red[1][warp] = sum;
+            __syncthreads();
+            sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+            if (col < a.Dv) {
 #pragma unroll 8
-                for (int i = grp; i < n; i += groups) {
-                    const float4 o = *reinterpret_cast<const float4*>(part_o + place(i, r) * a.Dv + u * 4);
-                    const float w = weight[i];
+                for (int i = warp; i < n; i += 4) {
+                    const float4 o = *reinterpret_cast<const float4*>(part_o + place(i) * a.Dv + col);
+                    const float w = s_ml[i].x;
                     v.x += o.x * w;
                     v.y += o.y * w;
                     v.z += o.z * w;
                     v.w += o.w * w;
                 }
             }
-            if (groups > 1) {
-                s_o[threadIdx.x] = v;
-                __syncthreads();
-                if (grp == 0)
-                    for (int x = 1; x < groups; ++x) {
-                        const float4 o = s_o[x * units + u];
-                        v.x += o.x;
-                        v.y += o.y;
-                        v.z += o.z;
-                        v.w += o.w;
-                    }
-            }
-            if (grp == 0) store(tile_base + r, u * 4, v, sum);
+            s_o[threadIdx.x] = v;
+            __syncthreads();
+            if (warp == 0)
+#pragma unroll
+                for (int x = 1; x < 4; ++x) {
+                    const float4 o = s_o[x * 32 + lane];
+                    v.x += o.x;
+                    v.y += o.y;
+                    v.z += o.z;
+                    v.w += o.w;
+                }
         }
-        __syncthreads();
+        if (col < a.Dv && (!wide || warp == 0)) {
+            const int j = gr / G, hq = h * G + gr - j * G;
+            const int count = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
+            const bool none = j >= count || sum == 0.f;
+            const float inv = __fdividef(1.f, sum);
+            uint2 res;
+            res.x = none ? 0u : pack2<T>(v.x * inv, v.y * inv);
+            res.y = none ? 0u : pack2<T>(v.z * inv, v.w * inv);
+            *reinterpret_cast<uint2*>((T*)a.out + (((int64_t)b * a.S + j) * a.Hq + hq) * a.Dv + col) = res;
+        }
     }
 }
 
@@ -854,19 +861,18 @@ struct Workspace {
     }
 };
 
-template <typename T, int THREADS>
-static void launch_join(const AttnArgs& a, int rows, int per_block, int ctas, const Workspace& ws, cudaStream_t st) {
-    if (ctas < 2) return;
+template <typename T>
+static void launch_join(const AttnArgs& a, int rows, int ctas, const Workspace& ws, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(ctas - 1), (unsigned)ceil_div(std::min(rows, a.S * (a.Hq / a.Hkv)), per_block));
-    cfg.blockDim = dim3(THREADS);
+    cfg.gridDim = dim3((unsigned)at::cuda::getCurrentDeviceProperties()->multiProcessorCount * 4);
+    cfg.blockDim = dim3(128);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T, THREADS>, a, rows, per_block, (const int4*)ws.jobs, (const float*)ws.ml, (const float*)ws.o));
+    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T>, a, rows, ctas, (const int4*)ws.jobs, (const float*)ws.ml, (const float*)ws.o));
 }
 
 template <typename T, bool E4M3, int DP, int WR>
@@ -884,7 +890,7 @@ static void launch_rows(const AttnArgs& a, int64_t B, const at::Tensor& q) {
     cudaStream_t st = current_stream();
     rows_kernel<T, E4M3, DP, WR><<<ctas, 128, Sh::kSmem, st>>>(a, (int)B, ws.jobs, ws.ml, ws.o);
     ATB_LAUNCH_CHECK();
-    launch_join<T, 128>(a, rows, 4, ctas, ws, st);
+    launch_join<T>(a, rows, ctas, ws, st);
 }
 
 template <typename T, bool E4M3, int DP>
@@ -920,6 +926,7 @@ struct LatentShape {
     static constexpr int kScoreRow = 72;  // floats; 64 keys, spread over the banks
     static constexpr int kScores = kRing * kStageBytes;
     static constexpr int kProbs = kScores + 4 * 16 * MT * kScoreRow * 4;
+    static_assert(4 * kScoreRow * 4 == kJoint * 2, "the queries pass through the scores' memory");
     static constexpr int kSmem = kProbs + 16 * MT * 128;
 };
 
@@ -1025,25 +1032,30 @@ __global__ void __launch_bounds__(256) latent_kernel(const AttnArgs a, int B, in
             look_up(t + 1);
         }
 
-        // this warp's depth slice of the queries
-        auto q_src = [&](int r, int col) -> const T* {  // element `col` of the joint row of query row r, or null
-            const int gr = tile_base + r;
-            if (gr >= M) return nullptr;
-            const int j = gr / H, h = gr - j * H;
-            if (col < kLatent) return col < a.D1 ? (const T*)a.q + b * a.q_b + j * a.q_s + h * a.q_h + col : nullptr;
-            return col - kLatent < a.D - a.D1 ? (const T*)a.q2 + b * a.q2_b + j * a.q2_s + h * a.q2_h + col - kLatent : nullptr;
-        };
-        // |scale| log2 e and, for bf16 queries against an 8-bit cache, the inverse of the row's power of two (see above)
-        float up[MT][2];
+        // The queries pass through the score rows' memory (of the same size): joint rows [latent | rotary] with zeros where
+        // there is no row or a width is narrower.
+        {
+            constexpr int kQChunks = kJoint / 8;
+            for (int x = tid; x < kRows * kQChunks; x += 256) {
+                const int r = x / kQChunks, ch = x - r * kQChunks, gr = tile_base + r, col = ch * 8;
+                const int j = min(gr, M - 1) / H, h = min(gr, M - 1) - j * H;
+                const T* src = col < kLatent ? (const T*)a.q + b * a.q_b + j * a.q_s + h * a.q_h + col
+                                             : (const T*)a.q2 + b * a.q2_b + j * a.q2_s + h * a.q2_h + col - kLatent;
+                const bool full = gr < M && (col < kLatent ? col < a.D1 : col - kLatent < a.D - a.D1);
+                copy16(ring + Sh::kScores + r * (kJoint * 2) + ((ch ^ (r & 7)) * 16), full ? (const void*)src : a.q, full);
+            }
+            copies_commit();
+            copies_wait<0>();
+            __syncthreads();
+        }
+        const uint8_t* q_rows = smem + Sh::kScores;
+        // bf16 queries against an 8-bit cache: the row's power of two (see the grouped form)
         if (E4M3 && std::is_same<T, bf16>::value) {
             for (int r = warp; r < kRows; r += 8) {
                 float m = 0.f;
-                for (int col = lane * 2; col < kJoint; col += 64) {
-                    const T* src = q_src(r, col);
-                    if (src) {
-                        const float2 x = unpack2<T>(*reinterpret_cast<const uint32_t*>(src));
-                        m = fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y)));
-                    }
+                for (int x = lane; x < kJoint / 2; x += 32) {
+                    const float2 y = unpack2<T>(*reinterpret_cast<const uint32_t*>(q_rows + r * (kJoint * 2) + x * 4));
+                    m = fmaxf(m, fmaxf(fabsf(y.x), fabsf(y.y)));
                 }
                 m = warp_max(m);
                 const int e = (__float_as_uint(m) >> 23) & 255;
@@ -1051,30 +1063,26 @@ __global__ void __launch_bounds__(256) latent_kernel(const AttnArgs a, int B, in
             }
             __syncthreads();
         }
+        // this warp's depth slice of them
         uint32_t q[MT][kSteps][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = mt * 16 + g + 8 * i;
-                if (E4M3 && std::is_same<T, bf16>::value) up[mt][i] = s_fac[r];
+                const uint8_t* row = q_rows + r * (kJoint * 2);
+                const float up = E4M3 && std::is_same<T, bf16>::value ? s_fac[r] : 1.f;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
-                    const int col = (dg * kSteps + k) * 16;
-                    uint32_t x = 0, y = 0;
-                    if (E4M3) {
-                        const T* src = q_src(r, col);
-                        if (src) {
-                            const uint2 u = *reinterpret_cast<const uint2*>(src + 4 * c);
-                            x = u.x;
-                            y = u.y;
-                        }
+                    const int ch = (dg * kSteps + k) * 2;
+                    uint32_t x, y;
+                    if (E4M3) {  // elements 4 c .. 4 c + 3, the order in which the keys' bytes arrive
+                        const uint2 u = *reinterpret_cast<const uint2*>(row + (((ch + (c >> 1)) ^ (r & 7)) * 16) + (c & 1) * 8);
+                        x = u.x;
+                        y = u.y;
                     } else {
-                        const T* src = q_src(r, col);
-                        if (src) {
-                            x = *reinterpret_cast<const uint32_t*>(src + 2 * c);
-                            y = *reinterpret_cast<const uint32_t*>(src + 8 + 2 * c);
-                        }
+                        x = *reinterpret_cast<const uint32_t*>(row + ((ch ^ (r & 7)) * 16) + c * 4);
+                        y = *reinterpret_cast<const uint32_t*>(row + (((ch + 1) ^ (r & 7)) * 16) + c * 4);
                     }
                     if (a.scale < 0.f) {
                         x ^= 0x80008000u;
@@ -1082,8 +1090,8 @@ __global__ void __launch_bounds__(256) latent_kernel(const AttnArgs a, int B, in
                     }
                     if (E4M3 && std::is_same<T, bf16>::value) {
                         const float2 fx = unpack2<T>(x), fy = unpack2<T>(y);
-                        x = pack2<__half>(fx.x * up[mt][i], fx.y * up[mt][i]);
-                        y = pack2<__half>(fy.x * up[mt][i], fy.y * up[mt][i]);
+                        x = pack2<__half>(fx.x * up, fx.y * up);
+                        y = pack2<__half>(fy.x * up, fy.y * up);
                     }
                     q[mt][k][i] = x;
                     q[mt][k][i + 2] = y;
@@ -1389,7 +1397,7 @@ static void launch_latent_rows(const AttnArgs& a, int64_t B, const at::Tensor& q
     cudaStream_t st = current_stream();
     latent_kernel<T, E4M3, MT><<<ctas, 256, Sh::kSmem, st>>>(a, (int)B, ws.jobs, ws.ml, ws.o);
     ATB_LAUNCH_CHECK();
-    launch_join<T, 256>(a, rows, 1, ctas, ws, st);
+    launch_join<T>(a, rows, ctas, ws, st);
 }
 
 template <typename T, bool E4M3>
