@@ -718,22 +718,23 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, int4
 }
 
 // Adds the pieces of an item that several CTAs of the attention kernel worked on, in their order along the keys.  Such an item
-// lies across the begin of some CTA's piece; the attention kernel left a job there.  Every block gathers the jobs (their order
-// does not matter) and the blocks share out (job, query row, 128 columns): a warp each where the items have few pieces, a block
+// lies across the begin of some CTA's piece; the attention kernel left a job there.  Every block gathers the jobs, all in the
+// same order, and the blocks share out (job, query row, 128 columns): a warp each where the items have few pieces, a block
 // each, its warps taking pieces in turn, where some item has many.  The kernel is launched while the attention kernel runs, and
-// waits for its end before it reads.
+// waits for its end before it reads.  (Its pointers are not declared free of aliases: loads that are known to be invariant may
+// be moved ahead of the wait.)
 constexpr int kMaxCtas = 1024;
 template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int rows, int ctas, const int4* __restrict__ jobs,
-                                                   const float* __restrict__ part_ml, const float* __restrict__ part_o) {
+__global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int rows, int ctas, const int4* jobs, const float* part_ml,
+                                                   const float* part_o) {
     __shared__ int4 s_jobs[kMaxCtas];
-    __shared__ int s_first[kMaxCtas], s_count, s_most;
+    __shared__ int s_first[kMaxCtas], s_place[32], s_most;
     __shared__ float2 s_ml[kMaxCtas];
     __shared__ float s_red[2][4];
     __shared__ float4 s_o[128];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int G = a.Hq / a.Hkv, M = a.S * G, row_tiles = (M + rows - 1) / rows;
-    if (threadIdx.x == 0) s_count = s_most = 0;
+    if (threadIdx.x == 0) s_most = 0;
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int4 mine[kMaxCtas / 128];
@@ -742,17 +743,34 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int rows, i
         const int k = threadIdx.x + 128 * x;
         mine[x] = k < ctas ? jobs[k] : make_int4(0, 0, 0, 0);
     }
+    static_assert(kMaxCtas / 128 * 4 <= 32, "one lane per warp and round");
+    uint32_t has[kMaxCtas / 128];
 #pragma unroll
-    for (int x = 0; x < kMaxCtas / 128; ++x)
+    for (int x = 0; x < kMaxCtas / 128; ++x) {
+        has[x] = __ballot_sync(0xffffffffu, mine[x].z > 0);
+        if (lane == 0) s_place[x * 4 + warp] = __popc(has[x]);
+    }
+    __syncthreads();
+    int upto = s_place[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    const int n_jobs = __shfl_sync(0xffffffffu, upto, 31);
+#pragma unroll
+    for (int x = 0; x < kMaxCtas / 128; ++x) {
+        const int base = __shfl_sync(0xffffffffu, upto, x * 4 + warp) - __popc(has[x]);
         if (mine[x].z > 0) {
-            const int at = atomicAdd(&s_count, 1);
+            const int at = base + __popc(has[x] & ((1u << lane) - 1));
             s_jobs[at] = mine[x];
             s_first[at] = threadIdx.x + 128 * x - 1;
             atomicMax(&s_most, mine[x].z);
         }
+    }
     __syncthreads();
     const int used = row_tiles > 1 ? rows : M, slices = (a.Dv / 4 + 31) / 32;
-    const int total = s_count * used * slices;
+    const int total = n_jobs * used * slices;
     const bool wide = s_most > 8;  // a block for each unit
     for (int u = wide ? blockIdx.x : blockIdx.x * 4 + warp; u < total; u += wide ? gridDim.x : gridDim.x * 4) {
         const int col = (u % slices) * 128 + lane * 4, rest = u / slices;
