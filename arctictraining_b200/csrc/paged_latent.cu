@@ -1,0 +1,1065 @@
+// SPDX-License-Identifier: Apache-2.0
+// Attention of new tokens over the paged latent cache (absorbed multi-head latent attention).
+#include "paged_attention.cuh"
+#include "ptx_sm100.cuh"
+
+namespace atb {
+
+at::Tensor& gemm_error_flag(const at::Device& dev);
+
+namespace paged {
+
+// ---- latent attention --------------------------------------------------------------------------------------------------
+// One key row [latent | rotary] for all heads, the latent being its value too: a row of 1152 bytes meets 2 x 16 MT query
+// rows' products, so with 16 heads and one new token the memory still sets the pace.  A CTA of eight warps keeps the
+// weighted values of its query rows in registers, 64 columns a warp, and takes 64 keys at a time.  Scores: the 36 depth
+// steps of 16 are divided over four groups of warps (whose slice of the queries stays in registers) and the keys over two, so
+// every key byte is read from shared memory once; the four partial sums meet in shared memory, where the softmax is taken by
+// all threads.  Weighted values: every warp reads its own 64 columns of the same tile.  Precision is that of the grouped form.
+constexpr int kLatent = 512, kRotary = 64, kJoint = kLatent + kRotary;
+
+template <bool E4M3, int MT>
+struct LatentShape {
+    static constexpr int kKeys = 64;
+    static constexpr int kRowBytes = kJoint * (E4M3 ? 1 : 2);
+    static constexpr int kStageBytes = kKeys * kRowBytes + (E4M3 ? kKeys * 4 : 0);
+    static constexpr int kRing = E4M3 ? 4 : 2;
+    static constexpr int kScoreRow = 72;  // floats; 64 keys, spread over the banks
+    static constexpr int kScores = kRing * kStageBytes;
+    static constexpr int kProbs = kScores + 4 * 16 * MT * kScoreRow * 4;
+    static_assert(4 * kScoreRow * 4 == kJoint * 2, "the queries pass through the scores' memory");
+    static constexpr int kSmem = kProbs + 16 * MT * 128;
+};
+
+template <typename T, bool E4M3, int MT>
+__global__ void __launch_bounds__(256) latent_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __restrict__ part_ml,
+                                                    float* __restrict__ part_o) {
+    using Sh = LatentShape<E4M3, MT>;
+    using P = typename std::conditional<E4M3, __half, T>::type;
+    constexpr int NK = Sh::kKeys, RB = Sh::kRowBytes, CPR = RB / 16, kRing = Sh::kRing, kRows = 16 * MT;
+    constexpr int kSteps = 9;            // depth steps of a warp
+    constexpr int kVal = E4M3 ? 8 : 4;   // registers of two 16-byte chunks of 16 values
+    constexpr int kVChunks = 64 * (E4M3 ? 1 : 2) / 16;  // a warp's chunks of a value row
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int scratch[10];
+    __shared__ uint32_t s_valid[kRing][2];
+    __shared__ float s_grow[kRows], s_fac[kRows], s_m[kRows], s_l[kRows];
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int dg = warp & 3, kh = warp >> 2;
+    const int H = a.Hq, M = a.S * H, per = (M + kRows - 1) / kRows;
+
+    int b, line, at, to;
+    const Pieces pieces = find_piece<256>(a, B, NK, per, gridDim.x, blockIdx.x, at, to, b, line, scratch);
+    Range rg;
+    if (at < to) rg = seq_range(a, b, NK);
+    if (threadIdx.x == 0) jobs[blockIdx.x] = join_job(a, pieces, blockIdx.x, at, to, b, line, rg);
+    if (at >= to) return;
+    const int began = at;
+    const uint32_t ring = smem_addr(smem);
+    float* scores = reinterpret_cast<float*>(smem + Sh::kScores);
+    const uint32_t probs = smem_addr(smem) + Sh::kProbs;
+    // place of a 16-byte chunk in a row: exchanged by the row's low bits so that eight rows meet different banks
+    auto chunk_at = [](int key, int ch) { return (E4M3 ? ch ^ ((key >> 1) & 3) : ch ^ (key & 7)) * 16; };
+
+    while (at < to) {
+        while (at >= line + rg.rounds * per) {
+            line += rg.rounds * per;
+            ++b;
+            rg = seq_range(a, b, NK);
+        }
+        const int item = (at - line) / rg.rounds;
+        const int v0 = at - line - item * rg.rounds, v1 = min(rg.rounds, v0 + (to - at));
+        const int r0 = max(0, v0 - a.lead), r1 = v1 - a.lead;
+        if (r1 <= r0) {
+            at += v1 - v0;
+            continue;
+        }
+        const int n = r1 - r0, tile_base = item * kRows;
+        const int* table = a.table + b * a.table_stride;
+
+        // copies of tile t: four threads a key
+        const int my_key = tid >> 2, my_part = tid & 3;
+        int look_w, look_off, look_key = rg.first + r0 * NK + my_key, pid_next;
+        look_w = look_key / a.page;
+        look_off = look_key - look_w * a.page;
+        const int step_w = NK / a.page, step_off = NK - step_w * a.page;
+        auto look_up = [&](int t) {
+            pid_next = -1;
+            if (t < n && look_key < rg.total) pid_next = table[look_w];
+        };
+        auto issue = [&](int t) {
+            if (t < n) {
+                const int st = t % kRing;
+                const uint32_t base = ring + st * Sh::kStageBytes + my_key * RB;
+                const bool ok = pid_next >= 0 && pid_next < a.P;
+                const uint8_t* src = (const uint8_t*)a.k_pages + (ok ? pid_next * a.k_page + (int64_t)look_off * a.D : 0) * (E4M3 ? 1 : 2);
+                const int lat = a.D1 * (E4M3 ? 1 : 2), all = a.D * (E4M3 ? 1 : 2);
+                constexpr int kLatChunks = kLatent * (E4M3 ? 1 : 2) / 16;
+#pragma unroll
+                for (int i = 0; i < CPR / 4; ++i) {
+                    const int ch = i * 4 + my_part;
+                    // narrower latents leave zeros between themselves and the rotary part
+                    const int byte = ch < kLatChunks ? ch * 16 : lat + (ch - kLatChunks) * 16;
+                    const bool full = ok && (ch < kLatChunks ? byte < lat : byte < all);
+                    copy16(base + chunk_at(my_key, ch), full ? src + byte : (const uint8_t*)a.k_pages, full);
+                }
+                if (E4M3 && my_part == 0)
+                    copy4(ring + st * Sh::kStageBytes + NK * RB + my_key * 4, a.k_scale + (ok ? pid_next * a.ks_page + look_off : 0), ok);
+                // eight keys a warp: their bits, gathered from the first lane of each
+                const uint32_t bits = __ballot_sync(0xffffffffu, ok);
+                if (lane == 0) {
+                    uint32_t eight = 0;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) eight |= ((bits >> (4 * k)) & 1u) << k;
+                    reinterpret_cast<uint8_t*>(s_valid[st])[warp] = (uint8_t)eight;
+                }
+                look_key += NK;
+                look_w += step_w;
+                look_off += step_off;
+                if (look_off >= a.page) {
+                    look_off -= a.page;
+                    ++look_w;
+                }
+            }
+            copies_commit();
+        };
+
+        look_up(0);
+#pragma unroll
+        for (int t = 0; t < kRing - 1; ++t) {
+            issue(t);
+            look_up(t + 1);
+        }
+
+        // The queries pass through the score rows' memory (of the same size): joint rows [latent | rotary] with zeros where
+        // there is no row or a width is narrower.
+        {
+            constexpr int kQChunks = kJoint / 8;
+            for (int x = tid; x < kRows * kQChunks; x += 256) {
+                const int r = x / kQChunks, ch = x - r * kQChunks, gr = tile_base + r, col = ch * 8;
+                const int j = min(gr, M - 1) / H, h = min(gr, M - 1) - j * H;
+                const T* src = col < kLatent ? (const T*)a.q + b * a.q_b + j * a.q_s + h * a.q_h + col
+                                             : (const T*)a.q2 + b * a.q2_b + j * a.q2_s + h * a.q2_h + col - kLatent;
+                const bool full = gr < M && (col < kLatent ? col < a.D1 : col - kLatent < a.D - a.D1);
+                copy16(ring + Sh::kScores + r * (kJoint * 2) + ((ch ^ (r & 7)) * 16), full ? (const void*)src : a.q, full);
+            }
+            copies_commit();
+            copies_wait<0>();
+            __syncthreads();
+        }
+        const uint8_t* q_rows = smem + Sh::kScores;
+        // bf16 queries against an 8-bit cache: the row's power of two (see the grouped form)
+        if (E4M3 && std::is_same<T, bf16>::value) {
+            for (int r = warp; r < kRows; r += 8) {
+                float m = 0.f;
+                for (int x = lane; x < kJoint / 2; x += 32) {
+                    const float2 y = unpack2<T>(*reinterpret_cast<const uint32_t*>(q_rows + r * (kJoint * 2) + x * 4));
+                    m = fmaxf(m, fmaxf(fabsf(y.x), fabsf(y.y)));
+                }
+                m = warp_max(m);
+                const int e = (__float_as_uint(m) >> 23) & 255;
+                if (lane == 0) s_fac[r] = __uint_as_float((uint32_t)(e == 0 || e == 255 ? 127 : min(268 - e, 253)) << 23);
+            }
+            __syncthreads();
+        }
+        // this warp's depth slice of them
+        uint32_t q[MT][kSteps][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = mt * 16 + g + 8 * i;
+                const uint8_t* row = q_rows + r * (kJoint * 2);
+                const float up = E4M3 && std::is_same<T, bf16>::value ? s_fac[r] : 1.f;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    const int ch = (dg * kSteps + k) * 2;
+                    uint32_t x, y;
+                    if (E4M3) {  // elements 4 c .. 4 c + 3, the order in which the keys' bytes arrive
+                        const uint2 u = *reinterpret_cast<const uint2*>(row + (((ch + (c >> 1)) ^ (r & 7)) * 16) + (c & 1) * 8);
+                        x = u.x;
+                        y = u.y;
+                    } else {
+                        x = *reinterpret_cast<const uint32_t*>(row + ((ch ^ (r & 7)) * 16) + c * 4);
+                        y = *reinterpret_cast<const uint32_t*>(row + (((ch + 1) ^ (r & 7)) * 16) + c * 4);
+                    }
+                    if (a.scale < 0.f) {
+                        x ^= 0x80008000u;
+                        y ^= 0x80008000u;
+                    }
+                    if (E4M3 && std::is_same<T, bf16>::value) {
+                        const float2 fx = unpack2<T>(x), fy = unpack2<T>(y);
+                        x = pack2<__half>(fx.x * up, fx.y * up);
+                        y = pack2<__half>(fy.x * up, fy.y * up);
+                    }
+                    q[mt][k][i] = x;
+                    q[mt][k][i + 2] = y;
+                }
+            }
+
+        // softmax: kLanes threads a row, kCols keys each
+        constexpr int kLanes = 256 / kRows, kCols = NK / kLanes;
+        const int srow = tid / kLanes, scol = (tid % kLanes) * kCols;
+        const int sj = min(tile_base + srow, M - 1) / H;
+        const int hi = (int)min((int64_t)rg.start + sj, (int64_t)rg.total - 1);
+        float fac = fmaxf(fabsf(a.scale), 1e-30f) * kLog2e;
+        if (E4M3 && std::is_same<T, bf16>::value) fac *= __uint_as_float((254u << 23) - __float_as_uint(s_fac[srow]));
+        float m = -INFINITY, mv = -INFINITY, l = 0.f;
+        float o[MT][8][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[mt][i][x] = 0.f;
+
+        for (int t = 0; t < n; ++t) {
+            copies_wait<kRing - 2>();
+            __syncthreads();  // tile t is here; every warp is done with tile t - 1
+            issue(t + kRing - 1);
+            look_up(t + kRing);
+            const int st = t % kRing;
+            const uint32_t base = ring + st * Sh::kStageBytes;
+            const int first = rg.first + (r0 + t) * NK;
+            // scores of this warp's 32 keys and depth slice
+            {
+                float s[MT][4][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) s[mt][i][x] = 0.f;
+                const int r = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1;
+#pragma unroll
+                for (int kp = 0; kp < 2; ++kp) {
+                    const int key = kh * 32 + kp * 16 + r;
+                    const uint32_t krow = base + key * RB;
+                    if (E4M3) {
+#pragma unroll
+                        for (int k = 0; k < kSteps; k += 2) {
+                            uint32_t f[4];
+                            // the ninth step has no partner: its second half is read again and not used
+                            const int ch = dg * kSteps + min(k + half, kSteps - 1);
+                            ldsm4(f, krow + chunk_at(key, ch));
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                if (k + (x & 1) >= kSteps) continue;
+                                uint32_t b0, b1;
+                                e4m3x4_to_f16x4(f[x], b0, b1);
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) mma<P>(s[mt][2 * kp + (x >> 1)], q[mt][k + (x & 1)], b0, b1);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < kSteps; ++k) {
+                            uint32_t f[4];
+                            ldsm4(f, krow + chunk_at(key, 2 * (dg * kSteps + k) + half));
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                mma<P>(s[mt][2 * kp], q[mt][k], f[0], f[1]);
+                                mma<P>(s[mt][2 * kp + 1], q[mt][k], f[2], f[3]);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float* dst = scores + (dg * kRows + mt * 16 + g) * Sh::kScoreRow + kh * 32 + i * 8 + 2 * c;
+                        *reinterpret_cast<float2*>(dst) = make_float2(s[mt][i][0], s[mt][i][1]);
+                        *reinterpret_cast<float2*>(dst + 8 * Sh::kScoreRow) = make_float2(s[mt][i][2], s[mt][i][3]);
+                    }
+            }
+            __syncthreads();
+            // softmax of the tile
+            {
+                float x[kCols], lv[kCols];
+#pragma unroll
+                for (int i = 0; i < kCols; i += 4) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        const float4 y = *reinterpret_cast<const float4*>(scores + (d * kRows + srow) * Sh::kScoreRow + scol + i);
+                        v.x += y.x;
+                        v.y += y.y;
+                        v.z += y.z;
+                        v.w += y.w;
+                    }
+                    x[i] = v.x * fac;
+                    x[i + 1] = v.y * fac;
+                    x[i + 2] = v.z * fac;
+                    x[i + 3] = v.w * fac;
+                }
+                if (E4M3) {
+                    const float* sc = reinterpret_cast<const float*>(smem + st * Sh::kStageBytes + NK * RB) + scol;
+#pragma unroll
+                    for (int i = 0; i < kCols; ++i) {
+                        const float y = sc[i];
+                        x[i] *= y;
+                        lv[i] = __log2f(y);
+                    }
+                }
+                const uint32_t valid = s_valid[st][scol >> 5] >> (scol & 31);
+                float tm = -INFINITY, tv = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) {
+                    if (first + scol + i > hi || !((valid >> i) & 1)) x[i] = -INFINITY;
+                    tm = fmaxf(tm, x[i]);
+                    if (E4M3) tv = fmaxf(tv, x[i] + lv[i]);
+                }
+#pragma unroll
+                for (int d = 1; d < kLanes; d <<= 1) {
+                    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, d));
+                    if (E4M3) tv = fmaxf(tv, __shfl_xor_sync(0xffffffffu, tv, d));
+                }
+                if (!E4M3) tv = tm;
+                const float mn = fmaxf(m, tm), vn = fmaxf(mv, tv);
+                l *= m == -INFINITY ? 0.f : exp2f(m - mn);
+                if (tid % kLanes == 0) s_grow[srow] = mv == -INFINITY ? 0.f : exp2f(mv - vn);
+                m = mn;
+                mv = vn;
+                const float mz = m == -INFINITY ? 0.f : m, vz = mv == -INFINITY ? 0.f : mv;
+                uint32_t w[kCols / 2];
+#pragma unroll
+                for (int i = 0; i < kCols; i += 2) {
+                    float e[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float pr = exp2f(x[i + k] - mz);
+                        l += pr;
+                        e[k] = !E4M3 ? pr : x[i + k] == -INFINITY ? 0.f : exp2f(x[i + k] + lv[i + k] - vz);
+                    }
+                    w[i / 2] = pack2<P>(e[0], e[1]);
+                }
+                uint8_t* dst = smem + Sh::kProbs + srow * 128;
+                const int ch = scol / 8;
+                if (kCols == 4) *reinterpret_cast<uint2*>(dst + ((ch ^ (srow & 7)) * 16) + (scol & 4) * 2) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint4*>(dst + ((ch ^ (srow & 7)) * 16)) = make_uint4(w[0], w[1], w[kCols / 2 - 2], w[kCols / 2 - 1]);
+            }
+            __syncthreads();
+            // weighted values of this warp's 64 columns
+            {
+                bool grew = false;
+                float f[MT][2];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        f[mt][i] = s_grow[mt * 16 + g + 8 * i];
+                        grew = grew || f[mt][i] != 1.f;
+                    }
+                if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) o[mt][i][x] *= f[mt][x >> 1];
+                }
+                auto load_probs = [&](int mt, int kp, uint32_t (&p)[4]) {
+                    const int r = mt * 16 + (lane & 15);
+                    ldsm4(p, probs + r * 128 + (((kp * 2 + (lane >> 4)) ^ (r & 7)) * 16));
+                };
+                auto load_values = [&](int kp, int k, uint32_t (&v)[kVal]) {
+                    const int key = kp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+                    uint32_t x[4];
+                    ldsm4_t(x, base + key * RB + chunk_at(key, warp * kVChunks + k + (lane >> 4)));
+                    if constexpr (E4M3) {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+                            e4m3x4_to_f16x4(__byte_perm(x[y], 0, 0x3120), v[(y >> 1) * 4 + (y & 1)], v[(y >> 1) * 4 + 2 + (y & 1)]);
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) v[y] = x[y];
+                    }
+                };
+                const bool hidden = a.S > 1 && first + NK - 1 > rg.start;
+                if (hidden && values_not_finite<P, kVal, 4, kVChunks>(load_values)) {
+                    // see the grouped form: each new token's rows get a product without the keys hidden from them
+                    const int last = min(tile_base + kRows - 1, M - 1) / H;
+                    for (int j = tile_base / H; j <= last; ++j) {
+                        const int hj = (int)min((int64_t)rg.start + j, (int64_t)rg.total - 1);
+#pragma unroll 1
+                        for (int kp = 0; kp < 4; ++kp) {
+                            uint32_t keep[2], p[MT][4];
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const int pos = first + kp * 16 + 8 * x + 2 * c;
+                                keep[x] = (pos <= hj ? 0xffffu : 0u) | (pos + 1 <= hj ? 0xffff0000u : 0u);
+                            }
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) load_probs(mt, kp, p[mt]);
+#pragma unroll
+                            for (int k = 0; k < kVChunks; k += 2) {
+                                uint32_t v[kVal];
+                                load_values(kp, k, v);
+#pragma unroll
+                                for (int x = 0; x < kVal / 2; ++x)
+#pragma unroll
+                                    for (int mt = 0; mt < MT; ++mt) {
+                                        float add[4] = {0.f, 0.f, 0.f, 0.f};
+                                        mma<P>(add, p[mt], v[2 * x] & keep[0], v[2 * x + 1] & keep[1]);
+#pragma unroll
+                                        for (int y = 0; y < 4; ++y)
+                                            if (min(tile_base + mt * 16 + g + 8 * (y >> 1), M - 1) / H == j) o[mt][k * (kVal / 4) + x][y] += add[y];
+                                    }
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int kp = 0; kp < 4; ++kp) {
+                        uint32_t p[MT][4];
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) load_probs(mt, kp, p[mt]);
+#pragma unroll
+                        for (int k = 0; k < kVChunks; k += 2) {
+                            uint32_t v[kVal];
+                            load_values(kp, k, v);
+#pragma unroll
+                            for (int x = 0; x < kVal / 2; ++x)
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) mma<P>(o[mt][k * (kVal / 4) + x], p[mt], v[2 * x], v[2 * x + 1]);
+                        }
+                    }
+                }
+            }
+        }
+        copies_wait<0>();
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        __syncthreads();  // the last tile's s_grow has been read
+        if (tid % kLanes == 0) {
+            s_m[srow] = m;
+            s_l[srow] = l;
+            s_grow[srow] = !E4M3 ? 1.f : mv == -INFINITY ? 0.f : exp2f(mv - m);  // weighted values are in units of 2^mv
+        }
+        __syncthreads();
+        const bool whole = r0 == 0 && v1 == rg.rounds;
+        const int slot = at == began ? 0 : 1;
+        const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * kRows;
+        const int count = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = mt * 16 + g + 8 * i, gr = tile_base + r;
+                if (gr >= M) continue;
+                const float f = s_grow[r], sum = s_l[r];
+                const bool none = gr / H >= count || sum == 0.f;
+                const float inv = whole ? __fdividef(f, sum) : f;
+                T* out = (T*)a.out + (((int64_t)b * a.S * H) + gr) * a.Dv;
+                float* dst = part_o + (part + r) * a.Dv;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // 16 columns: two tiles of eight, or (8-bit) of even and of odd columns
+                    const int col = warp * 64 + k * 16;
+                    if (col >= a.Dv) continue;
+                    float e[4] = {o[mt][2 * k][2 * i] * inv, o[mt][2 * k][2 * i + 1] * inv, o[mt][2 * k + 1][2 * i] * inv,
+                                  o[mt][2 * k + 1][2 * i + 1] * inv};
+                    const int at0 = E4M3 ? col + 4 * c : col + 2 * c, at1 = E4M3 ? at0 + 2 : at0 + 8;
+                    if (E4M3) {
+                        const float x = e[1];
+                        e[1] = e[2];
+                        e[2] = x;
+                    }
+                    if (whole) {
+                        *reinterpret_cast<uint32_t*>(out + at0) = none ? 0u : pack2<T>(e[0], e[1]);
+                        *reinterpret_cast<uint32_t*>(out + at1) = none ? 0u : pack2<T>(e[2], e[3]);
+                    } else {
+                        *reinterpret_cast<float2*>(dst + at0) = make_float2(e[0], e[1]);
+                        *reinterpret_cast<float2*>(dst + at1) = make_float2(e[2], e[3]);
+                    }
+                }
+                if (!whole && warp == 0 && c == 0) {
+                    part_ml[(part + r) * 2] = s_m[r];
+                    part_ml[(part + r) * 2 + 1] = sum;
+                }
+            }
+        at += v1 - v0;
+        __syncthreads();
+    }
+}
+
+template <typename T, bool E4M3, int MT>
+static void launch_latent_rows(AttnArgs a, int64_t B, const at::Tensor& q) {
+    using Sh = LatentShape<E4M3, MT>;
+    static std::atomic<uint64_t> done{0};
+    allow_smem_once(latent_kernel<T, E4M3, MT>, Sh::kSmem, done);
+    const int rows = 16 * MT, ctas = std::min(kMaxCtas, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+    const int64_t items = ceil_div((int64_t)a.S * a.Hq, rows);
+    ATB_ARG(B * items * (ceil_div((int64_t)a.W * a.page, Sh::kKeys) + 3) < (int64_t(1) << 31),
+            "paged_latent_attention: too many sequences, query rows or positions for one call");
+    a.cols = a.Dv;
+    a.halves = 1;
+    a.token_tiles = 0;
+    a.lead = 2;
+    const Workspace ws(q, ctas, rows, a.cols);
+    cudaStream_t st = current_stream();
+    latent_kernel<T, E4M3, MT><<<ctas, 256, Sh::kSmem, st>>>(a, (int)B, ws.jobs, ws.ml, ws.o);
+    ATB_LAUNCH_CHECK();
+    launch_join<T>(a, rows, ctas, ws, st);
+}
+
+// ---- latent attention of many heads -------------------------------------------------------------------------------------
+// With 64 heads or more a token's query rows fill the 128 rows of the tensor core's accumulator, and 242 multiply-adds a cached
+// byte (128 heads) make the matrix rate the bound.  One CTA takes the 128 rows of a token's heads and half of the 512 value
+// columns: weighted values 256, two score buffers of 32 keys, and 384 of the 576 query columns as left operand fill the 512
+// columns of tensor memory; the other 192 query columns and four stages of 32 keys lie in shared memory.  A left operand in
+// tensor memory is not read again from shared memory for each of the 36 depth steps, whose bandwidth bounds a product with
+// only 32 columns.  The price of halves is that both compute the scores: 1.5 times the multiply-adds of one CTA per row tile,
+// whose 512 value columns alone would fill tensor memory.
+// Warps 0-3: a query row a thread: scores out of tensor memory, softmax, probabilities back in their place.  Warps 4-7 fetch keys
+// (8-bit ones are turned into fp16 on the way).  Warp 8 issues the products; scores of the next tile run ahead of the values
+// of this one.  All keys that a row tile sees are the same for its rows (one token), so hidden keys are never fetched.
+// The accumulator is rescaled only when a row's maximum grew by more than 2^8.  All waits are bounded.
+namespace tc {
+constexpr int kThreads = 288, kKeys = 32, kRing = 4, kRows = 128, kCols = 256;
+constexpr int kSub = kKeys * 128;                       // 64 columns of a stage, 128-byte swizzled rows
+constexpr int kStage = kJoint / 64 * kSub;
+constexpr int kQTmem = 384, kQSub = kRows * 128;        // query columns in tensor memory; 64 columns of the others
+constexpr int kQ = 0, kK = (kJoint - kQTmem) / 64 * kQSub, kScale = kK + kRing * kStage, kValid = kScale + kRing * kKeys * 4;
+constexpr int kBars = kValid + kRing * 4 + 8, kSmem = kBars + 32 * 8 + 64;
+static_assert(kBars % 8 == 0 && kK % 1024 == 0, "aligned");
+constexpr uint32_t kS = 256, kQCol = 320;               // columns of tensor memory: values 0, scores 256 and 288, queries 320
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr float kGrow = 8.f;
+
+struct Piece {
+    int b, item, r0, n, row0, rows, half, token;
+    bool whole, first;
+    Range rg;
+};
+// The pieces of one CTA in their order: every role walks the same ones.
+struct Walk {
+    int at, to, began, b, line, per;
+    Range rg;
+    __device__ __forceinline__ bool next(const AttnArgs& a, Piece& p) {
+        while (at < to) {
+            while (at >= line + rg.rounds * per) {
+                line += rg.rounds * per;
+                ++b;
+                rg = seq_range(a, b, kKeys);
+            }
+            p.item = (at - line) / rg.rounds;
+            const int v0 = at - line - p.item * rg.rounds, v1 = min(rg.rounds, v0 + (to - at));
+            p.first = at == began;
+            at += v1 - v0;
+            p.r0 = max(0, v0 - a.lead);
+            p.n = v1 - a.lead - p.r0;
+            if (p.n <= 0) continue;
+            p.b = b;
+            p.rg = rg;
+            p.whole = p.r0 == 0 && v1 == rg.rounds;
+            int h;
+            item_rows(a, p.item, kRows, h, p.half, p.row0, p.rows);
+            p.token = p.row0 / a.Hq;
+            return true;
+        }
+        return false;
+    }
+};
+
+template <typename Q, bool E4M3>
+__global__ void __launch_bounds__(kThreads, 1)
+latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __restrict__ part_ml, float* __restrict__ part_o, int* error_flag) {
+    using P = typename std::conditional<E4M3, __half, Q>::type;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    int* scratch = reinterpret_cast<int*>(smem + kBars + 32 * 8);  // no static memory: the tiles' alignment
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBars);
+    uint64_t *k_full = bars, *k_empty = bars + kRing, *s_full = bars + 2 * kRing, *p_full = s_full + 2, *pv_done = p_full + 2,
+             *q_full = pv_done + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* s_scale = reinterpret_cast<float*>(smem + kScale);
+    uint32_t* s_valid = reinterpret_cast<uint32_t*>(smem + kValid);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    Walk walk;
+    walk.per = a.S * a.token_tiles * a.halves;
+    const Pieces pieces = find_piece<kThreads>(a, B, kKeys, walk.per, gridDim.x, blockIdx.x, walk.at, walk.to, walk.b, walk.line, scratch);
+    if (walk.at < walk.to) walk.rg = seq_range(a, walk.b, kKeys);
+    if (threadIdx.x == 0) jobs[blockIdx.x] = join_job(a, pieces, blockIdx.x, walk.at, walk.to, walk.b, walk.line, walk.rg);
+    if (walk.at >= walk.to) return;
+    walk.began = walk.at;
+    if ((ptx::smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need 1024-byte alignment
+        if (threadIdx.x == 0) atomicCAS(error_flag, 0, (0x30 << 8) | 1);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kRing; ++i) {
+            ptx::mbar_init(&k_full[i], 128);
+            ptx::mbar_init(&k_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&s_full[i], 1);
+            ptx::mbar_init(&p_full[i], 128);
+            ptx::mbar_init(&pv_done[i], 1);
+        }
+        ptx::mbar_init(q_full, 128);
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async_smem();
+    }
+    if (warp == 8) {
+        ptx::tmem_alloc(tmem_slot, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    Piece p;
+
+    if (warp >= 4 && warp < 8) {
+        // -------------------------------------------------------------------------------- keys: four threads a row
+        const int tid = threadIdx.x - 128, key = tid >> 2, part = tid & 3;
+        bool ok = true, more = walk.next(a, p);
+        int t_in = 0, pos = 0, w = 0, off = 0, pid = -1, upto = 0;
+        const int step_w = kKeys / a.page, step_off = kKeys - step_w * a.page;
+        auto look_up = [&]() { pid = pos < upto ? a.table[p.b * a.table_stride + w] : -1; };
+        auto begin_piece = [&]() {
+            t_in = 0;
+            upto = (int)min((int64_t)p.rg.total, (int64_t)p.rg.start + p.token + 1);
+            pos = p.rg.first + p.r0 * kKeys + key;
+            w = pos / a.page;
+            off = pos - w * a.page;
+            look_up();
+        };
+        if (more) begin_piece();
+        // source of this thread's row of the next tile, which then moves on
+        const uint8_t* src = nullptr;
+        const float* scale_src = nullptr;
+        bool full = false;
+        auto next_tile = [&]() {
+            full = pid >= 0 && pid < a.P;
+            const int64_t row = full ? pid * a.k_page + (int64_t)off * kJoint : 0;
+            src = (const uint8_t*)a.k_pages + row * (E4M3 ? 1 : 2);
+            if (E4M3) scale_src = a.k_scale + (full ? pid * a.ks_page + off : 0);
+            pos += kKeys;
+            w += step_w;
+            off += step_off;
+            if (off >= a.page) {
+                off -= a.page;
+                ++w;
+            }
+            if (++t_in < p.n) look_up();
+            else if ((more = walk.next(a, p))) begin_piece();
+        };
+        auto place = [&](int st, int col) {  // of 16 bytes (8 elements) of this row
+            return smem + kK + st * kStage + (col >> 6) * kSub + key * 128 + ((((col >> 3) & 7) ^ (key & 7)) << 4);
+        };
+        auto mark = [&](int st, bool here) {  // the tile's keys that exist
+            const uint32_t bits = __ballot_sync(0xffffffffu, here);
+            if (lane == 0) {
+                uint32_t eight = 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) eight |= ((bits >> (4 * k)) & 1u) << k;
+                reinterpret_cast<uint8_t*>(s_valid + st)[warp - 4] = (uint8_t)eight;
+            }
+        };
+        int T = 0;
+        if constexpr (!E4M3) {
+            constexpr int kLag = 2;  // tiles whose copies are on their way
+            for (; more && ok; ++T) {
+                next_tile();
+                const int st = T % kRing;
+                ok = ptx::mbar_wait_bounded(&k_empty[st], ((T / kRing) & 1) ^ 1u, abort_flag, kWaitNs);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                mark(st, full);
+#pragma unroll
+                for (int i = 0; i < kJoint / 32; ++i) {
+                    const int col = (i * 4 + part) * 8;
+                    copy16(ptx::smem_u32(place(st, col)), full ? src + col * 2 : (const uint8_t*)a.k_pages, full);
+                }
+                copies_commit();
+                if (T >= kLag) {
+                    copies_wait<kLag>();
+                    ptx::fence_proxy_async_smem();
+                    ptx::mbar_arrive(&k_full[(T - kLag) % kRing]);
+                }
+            }
+            copies_wait<0>();
+            ptx::fence_proxy_async_smem();
+            if (ok)
+                for (int x = max(0, T - kLag); x < T; ++x) ptx::mbar_arrive(&k_full[x % kRing]);
+        } else {
+            uint4 now[9], ahead[9];
+            float scale_now = 0.f, scale_ahead = 0.f;
+            bool full_ahead = false;
+            auto fetch = [&]() {
+                next_tile();
+                full_ahead = full;
+                scale_ahead = part == 0 && full ? *scale_src : 0.f;
+#pragma unroll
+                for (int i = 0; i < 9; ++i)
+                    ahead[i] = full ? *reinterpret_cast<const uint4*>(src + (i * 4 + part) * 16) : make_uint4(0, 0, 0, 0);
+            };
+            bool loaded = more;
+            if (more) fetch();
+            for (; loaded && ok; ++T) {
+                const bool here = full_ahead;
+                scale_now = scale_ahead;
+#pragma unroll
+                for (int i = 0; i < 9; ++i) now[i] = ahead[i];
+                loaded = more;
+                if (more) fetch();
+                const int st = T % kRing;
+                ok = ptx::mbar_wait_bounded(&k_empty[st], ((T / kRing) & 1) ^ 1u, abort_flag, kWaitNs);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                mark(st, here);
+                if (part == 0) s_scale[st * kKeys + key] = scale_now;
+#pragma unroll
+                for (int i = 0; i < 9; ++i) {
+                    const int col = (i * 4 + part) * 16;
+                    uint4 lo, hi;
+                    e4m3x4_to_f16x4(now[i].x, lo.x, lo.y);
+                    e4m3x4_to_f16x4(now[i].y, lo.z, lo.w);
+                    e4m3x4_to_f16x4(now[i].z, hi.x, hi.y);
+                    e4m3x4_to_f16x4(now[i].w, hi.z, hi.w);
+                    *reinterpret_cast<uint4*>(place(st, col)) = lo;
+                    *reinterpret_cast<uint4*>(place(st, col + 8)) = hi;
+                }
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(&k_full[st]);
+            }
+        }
+        if (!ok && lane == 0) atomicCAS(error_flag, 0, (0x31 << 8) | 1);
+    } else if (warp == 8) {
+        // -------------------------------------------------------------------------------- products
+        if (lane == 0) {
+            constexpr uint32_t fmt = std::is_same<P, bf16>::value ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t kind = ~((1u << 7) | (1u << 10));
+            constexpr uint32_t idesc_qk = (ptx::make_idesc_bf16(kRows, kKeys, false, false) & kind) | fmt;
+            constexpr uint32_t idesc_pv = (ptx::make_idesc_bf16(kRows, kCols, false, true) & kind) | fmt;
+            const uint32_t qs = ptx::smem_u32(smem + kQ), ks0 = ptx::smem_u32(smem + kK);
+            int T = 0, np = 0;
+            bool ok = true;
+            auto issue_values = [&](int t, bool add, int half) -> bool {
+                if (!ptx::mbar_wait_bounded(&p_full[t & 1], (t >> 1) & 1, abort_flag, kWaitNs)) return false;
+                ptx::tc_fence_after();
+                const uint32_t vs = ks0 + (t % kRing) * kStage + half * (kCols / 64) * kSub;
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k)
+                    ptx::mma_bf16_ts(tmem, tmem + kS + (t & 1) * kKeys + k * 8, ptx::make_smem_desc_sw128(vs + k * 2048, kSub, 1024), idesc_pv,
+                                     add || k > 0);
+                ptx::mma_commit(&k_empty[t % kRing]);
+                ptx::mma_commit(&pv_done[t & 1]);
+                return true;
+            };
+            while (ok && walk.next(a, p)) {
+                ok = ptx::mbar_wait_bounded(q_full, np & 1, abort_flag, kWaitNs);
+                ++np;
+                for (int t = 0; t < p.n && ok; ++t, ++T) {
+                    ok = ptx::mbar_wait_bounded(&k_full[T % kRing], (T / kRing) & 1, abort_flag, kWaitNs);
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                    const uint32_t ks = ks0 + (T % kRing) * kStage, d = tmem + kS + (T & 1) * kKeys;
+#pragma unroll
+                    for (int k = 0; k < kJoint / 16; ++k) {
+                        const uint64_t kd = ptx::make_smem_desc_sw128(ks + (k >> 2) * kSub + (k & 3) * 32, 16, 1024);
+                        if (k < kQTmem / 16) ptx::mma_bf16_ts(d, tmem + kQCol + k * 8, kd, idesc_qk, k > 0);
+                        else ptx::mma_bf16_ss(d, ptx::make_smem_desc_sw128(qs + ((k - kQTmem / 16) >> 2) * kQSub + (k & 3) * 32, 16, 1024), kd, idesc_qk, 1u);
+                    }
+                    ptx::mma_commit(&s_full[T & 1]);
+                    if (t > 0) ok = issue_values(T - 1, t > 1, p.half);
+                }
+                if (ok) ok = issue_values(T - 1, p.n > 1, p.half);
+            }
+            if (!ok) atomicCAS(error_flag, 0, (0x32 << 8) | 1);
+        }
+    } else {
+        // -------------------------------------------------------------------------------- softmax: a query row a thread
+        const int r = threadIdx.x;
+        const uint32_t my = tmem + ((uint32_t)(warp * 32) << 16);
+        int T = 0;
+        bool ok = true;
+        // values of tile t are added: a barrier for even and one for odd tiles, since a wait names a phase by its parity only
+        // and the tile before may not be done either
+        auto values_done = [&](int t) {
+            return (bool)__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&pv_done[t & 1], (t >> 1) & 1, abort_flag, kWaitNs));
+        };
+        while (ok && walk.next(a, p)) {
+            // this row's queries: [latent | rotary], zeros where the tile has no row
+            const bool real = r < p.rows;
+            const int gr = p.row0 + (real ? r : 0), j = p.token, h = gr - j * a.Hq;
+            const Q* ql = (const Q*)a.q + p.b * a.q_b + j * a.q_s + h * a.q_h;
+            const Q* qr = (const Q*)a.q2 + p.b * a.q2_b + j * a.q2_s + h * a.q2_h;
+            float fac = fmaxf(fabsf(a.scale), 1e-30f) * kLog2e, up = 1.f;
+            auto load_q = [&](int col) -> uint4 {
+                if (!real) return make_uint4(0, 0, 0, 0);
+                return *reinterpret_cast<const uint4*>(col < kLatent ? ql + col : qr + col - kLatent);
+            };
+            if (E4M3 && std::is_same<Q, bf16>::value) {  // the row's power of two (see the grouped form)
+                float m = 0.f;
+#pragma unroll 8
+                for (int col = 0; col < kJoint; col += 8) {
+                    const uint4 u = load_q(col);
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 y = unpack2<Q>(w[i]);
+                        m = fmaxf(m, fmaxf(fabsf(y.x), fabsf(y.y)));
+                    }
+                }
+                const int e = (__float_as_uint(m) >> 23) & 255;
+                const int field = e == 0 || e == 255 ? 127 : min(268 - e, 253);
+                up = __uint_as_float((uint32_t)field << 23);
+                fac *= __uint_as_float((uint32_t)(254 - field) << 23);
+            }
+            const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+            auto turn = [&](uint32_t u) -> uint32_t {
+                u ^= sign;
+                if (E4M3 && std::is_same<Q, bf16>::value) {
+                    const float2 y = unpack2<Q>(u);
+                    u = pack2<__half>(y.x * up, y.y * up);
+                }
+                return u;
+            };
+#pragma unroll 1
+            for (int c = 0; c < kQTmem / 64; ++c) {
+                uint32_t v[32];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 u = load_q(c * 64 + i * 8);
+                    v[4 * i] = turn(u.x);
+                    v[4 * i + 1] = turn(u.y);
+                    v[4 * i + 2] = turn(u.z);
+                    v[4 * i + 3] = turn(u.w);
+                }
+                __syncwarp();
+                ptx::tmem_st_32x32b_x32(my + kQCol + c * 32, v);
+            }
+#pragma unroll 8
+            for (int i = 0; i < (kJoint - kQTmem) / 8; ++i) {
+                uint4 u = load_q(kQTmem + i * 8);
+                u.x = turn(u.x);
+                u.y = turn(u.y);
+                u.z = turn(u.z);
+                u.w = turn(u.w);
+                *reinterpret_cast<uint4*>(smem + kQ + (i >> 3) * kQSub + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = u;
+            }
+            __syncwarp();
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before();
+            ptx::fence_proxy_async_smem();
+            ptx::mbar_arrive(q_full);
+
+            float m = -INFINITY, mv = -INFINITY, l = 0.f;  // references of the sum and of the weighted values, in log2 units
+            for (int t = 0; t < p.n; ++t, ++T) {
+                const int st = T % kRing;
+                ok = ptx::mbar_wait_bounded(&k_full[st], (T / kRing) & 1, abort_flag, kWaitNs) &&
+                     ptx::mbar_wait_bounded(&s_full[T & 1], (T >> 1) & 1, abort_flag, kWaitNs);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                uint32_t s[32];
+                ptx::tmem_ld_32x32b_x32(my + kS + (T & 1) * kKeys, s);
+                ptx::tmem_ld_wait();
+                const uint32_t valid = s_valid[st];
+                float x[32], lv[E4M3 ? 32 : 1];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(s[i]) * fac;
+                if constexpr (E4M3) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 sc = *reinterpret_cast<const float4*>(s_scale + st * kKeys + i);
+                        x[i] *= sc.x;
+                        x[i + 1] *= sc.y;
+                        x[i + 2] *= sc.z;
+                        x[i + 3] *= sc.w;
+                        lv[i] = __log2f(sc.x);
+                        lv[i + 1] = __log2f(sc.y);
+                        lv[i + 2] = __log2f(sc.z);
+                        lv[i + 3] = __log2f(sc.w);
+                    }
+                }
+                if (valid != 0xffffffffu) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!((valid >> i) & 1)) x[i] = -INFINITY;
+                }
+                float t0 = -INFINITY, t1 = -INFINITY, v0 = -INFINITY, v1 = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    t0 = fmaxf(t0, x[i]);
+                    t1 = fmaxf(t1, x[i + 1]);
+                    if constexpr (E4M3) {
+                        v0 = fmaxf(v0, x[i] + lv[i]);
+                        v1 = fmaxf(v1, x[i + 1] + lv[i + 1]);
+                    }
+                }
+                const float tm = fmaxf(t0, t1), tv = E4M3 ? fmaxf(v0, v1) : tm;
+                if (tm > m + (m == -INFINITY ? 0.f : kGrow)) {
+                    l *= m == -INFINITY ? 0.f : exp2f(m - tm);
+                    m = tm;
+                }
+                const bool grow = tv > mv + (mv == -INFINITY ? 0.f : kGrow);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = !grow ? 1.f : mv == -INFINITY ? 0.f : exp2f(mv - tv);
+                    if (grow) mv = tv;
+                    if (t > 0) {
+                        ok = values_done(T - 1);
+                        if (!ok) break;
+                        ptx::tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < kCols; c += 32) {
+                            uint32_t v[32];
+                            ptx::tmem_ld_32x32b_x32(my + c, v);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                            ptx::tmem_st_32x32b_x32(my + c, v);
+                        }
+                    }
+                }
+                const float mz = m == -INFINITY ? 0.f : m, vz = mv == -INFINITY ? 0.f : mv;
+                uint32_t pr[16];
+                float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float e0 = exp2f(x[i] - mz), e1 = exp2f(x[i + 1] - mz);
+                    l0 += e0;
+                    l1 += e1;
+                    if constexpr (E4M3)
+                        pr[i / 2] = pack2<P>(x[i] == -INFINITY ? 0.f : exp2f(x[i] + lv[i] - vz),
+                                             x[i + 1] == -INFINITY ? 0.f : exp2f(x[i + 1] + lv[i + 1] - vz));
+                    else pr[i / 2] = pack2<P>(e0, e1);
+                }
+                l += l0 + l1;
+                ptx::tmem_st_32x32b_x16(my + kS + (T & 1) * kKeys, pr);
+                ptx::tmem_st_wait();
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(&p_full[T & 1]);
+            }
+            if (ok) ok = values_done(T - 1);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const int count = a.counts ? max(0, min(a.counts[p.b], a.S)) : a.S;
+            const bool none = j >= count || l == 0.f;
+            // a whole item is divided by its sum; a piece's values are brought to the units of its sum, 2^m
+            float f = E4M3 ? (mv == -INFINITY ? 0.f : exp2f(mv - m)) : 1.f;
+            if (p.whole) f = __fdividef(f, l);
+            const int64_t part = ((int64_t)blockIdx.x * 2 + (p.first ? 0 : 1)) * kRows + r;
+            Q* out = (Q*)a.out + ((int64_t)p.b * a.S * a.Hq + gr) * kLatent + p.half * kCols;
+#pragma unroll 1
+            for (int c = 0; c < kCols; c += 32) {
+                uint32_t v[32];
+                __syncwarp();
+                ptx::tmem_ld_32x32b_x32(my + c, v);
+                ptx::tmem_ld_wait();
+                if (!real) continue;
+                if (p.whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float e[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) e[k] = none ? 0.f : __uint_as_float(v[i + k]) * f;
+                        *reinterpret_cast<uint4*>(out + c + i) = Vec8<Q>::pack(e);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(part_o + part * kCols + c + i) =
+                            make_float4(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f, __uint_as_float(v[i + 2]) * f,
+                                        __uint_as_float(v[i + 3]) * f);
+                }
+            }
+            if (!p.whole && real) {
+                part_ml[part * 2] = m;
+                part_ml[part * 2 + 1] = l;
+            }
+            ptx::tc_fence_before();
+        }
+        if (!ok && lane == 0) atomicCAS(error_flag, 0, (0x33 << 8) | 1);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    if (warp == 8) {
+        __syncwarp();
+        ptx::tmem_dealloc(tmem, 512);
+    }
+}
+}  // namespace tc
+
+template <typename T, bool E4M3>
+static void launch_latent_tc(AttnArgs a, int64_t B, const at::Tensor& q) {
+    static std::atomic<uint64_t> done{0};
+    allow_smem_once(tc::latent_tc_kernel<T, E4M3>, tc::kSmem, done);
+    const int ctas = std::min(kMaxCtas, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+    a.halves = 2;
+    a.cols = tc::kCols;
+    a.token_tiles = (a.Hq + tc::kRows - 1) / tc::kRows;
+    a.lead = 8;
+    const int64_t items = (int64_t)a.S * a.token_tiles * a.halves;
+    ATB_ARG(B * items * (ceil_div((int64_t)a.W * a.page, tc::kKeys) + 1 + a.lead) < (int64_t(1) << 31),
+            "paged_latent_attention: too many sequences, query rows or positions for one call");
+    const Workspace ws(q, ctas, tc::kRows, a.cols);
+    cudaStream_t st = current_stream();
+    int* error = gemm_error_flag(q.device()).data_ptr<int>();
+    tc::latent_tc_kernel<T, E4M3><<<ctas, tc::kThreads, tc::kSmem, st>>>(a, (int)B, ws.jobs, ws.ml, ws.o, error);
+    ATB_LAUNCH_CHECK();
+    launch_join<T>(a, tc::kRows, ctas, ws, st);
+}
+
+template <typename T, bool E4M3>
+static void launch_latent(const AttnArgs& a, int64_t B, const at::Tensor& q) {
+    // MEASURE
+    if (a.Hq >= 64 && a.D1 == kLatent && a.D == kJoint) return launch_latent_tc<T, E4M3>(a, B, q);
+    if (a.S * a.Hq <= 16) launch_latent_rows<T, E4M3, 1>(a, B, q);
+    else launch_latent_rows<T, E4M3, 2>(a, B, q);
+}
+
+}  // namespace paged
+
+using namespace paged;
+
+at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& q_pe, const at::Tensor& pages, const at::Tensor& table,
+                                  const at::Tensor& starts, const c10::optional<at::Tensor>& counts,
+                                  const c10::optional<at::Tensor>& page_scale, double scale) {
+    const char* op = "paged_latent_attention";
+    ATB_ARG(q.dim() == 4 && q_pe.dim() == 4, op, ": q_latent and q_pe must be [batch, new tokens, heads, width]");
+    const int64_t B = q.size(0), S = q.size(1), H = q.size(2), R = q.size(3), rope = q_pe.size(3);
+    ATB_ARG(q_pe.size(0) == B && q_pe.size(1) == S && q_pe.size(2) == H, op, ": q_latent and q_pe differ in shape");
+    ATB_ARG(half_type(q) && q_pe.scalar_type() == q.scalar_type(), op, ": q_latent and q_pe must be bf16 or fp16, both of one type");
+    ATB_ARG(R % 16 == 0 && R > 0 && R <= 512 && rope % 16 == 0 && rope > 0 && rope <= 64, op,
+            ": the latent must be a multiple of 16 up to 512, the rotary part one up to 64");
+    ATB_ARG(q_pe.device() == q.device(), op, ": all tensors must be on one device");
+    check_pages(op, pages, page_scale, q);
+    ATB_ARG(pages.size(1) == 1 && pages.size(3) == R + rope, op, ": a latent cache is [pages, 1, page, latent + rotary]");
+    ATB_ARG(is_e4m3(pages) || pages.scalar_type() == q.scalar_type(), op, ": the cache must have the query's type or be e4m3");
+    check_table(op, table, starts, counts, pages, B);
+    ATB_ARG(B * S * H < (int64_t(1) << 31), op, ": too many query rows");
+    const c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor out = at::empty({B, S, H, R}, q.options());
+    if (out.numel() == 0) return out;
+    if (pages.size(0) == 0 || table.size(1) == 0) return out.zero_();
+    const at::Tensor qc = rows16(q), pc = rows16(q_pe);
+    AttnArgs a;
+    a.q = qc.data_ptr(); a.q2 = pc.data_ptr();
+    a.q_b = qc.stride(0); a.q_s = qc.stride(1); a.q_h = qc.stride(2);
+    a.q2_b = pc.stride(0); a.q2_s = pc.stride(1); a.q2_h = pc.stride(2);
+    a.k_pages = a.v_pages = pages.data_ptr();
+    a.k_scale = a.v_scale = ptr<float>(page_scale);
+    a.k_page = a.v_page = pages.stride(0);
+    a.ks_page = a.vs_page = page_scale.has_value() ? page_scale->stride(0) : 0;
+    a.out = out.data_ptr();
+    a.table = table.data_ptr<int>(); a.starts = starts.data_ptr<int>(); a.counts = ptr<int>(counts);
+    a.table_stride = table.stride(0);
+    a.S = (int)S; a.Hq = (int)H; a.Hkv = 1; a.D = (int)(R + rope); a.D1 = a.Dv = (int)R; a.P = (int)pages.size(0);
+    a.W = (int)table.size(1); a.page = (int)pages.size(2); a.window = 0; a.scale = (float)scale;
+    const bool f8 = is_e4m3(pages);
+    if (q.scalar_type() == at::kBFloat16) f8 ? launch_latent<bf16, true>(a, B, q) : launch_latent<bf16, false>(a, B, q);
+    else f8 ? launch_latent<__half, true>(a, B, q) : launch_latent<__half, false>(a, B, q);
+    return out;
+}
+
+}  // namespace atb

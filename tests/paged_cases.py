@@ -39,6 +39,12 @@ LATENT = {
     "many-heads": dict(starts=[100, 333], S=1, h=128, R=512, rope=64, page=64),
     "many-heads-draft": dict(starts=[5, 90], S=2, h=128, R=512, rope=64, page=64),
     "twenty-heads": dict(starts=[200, 10], S=3, h=20, R=512, rope=64, page=48),
+    "sixty-four-heads-draft": dict(starts=[200, 31, 0], S=3, h=64, R=512, rope=64, page=48),
+    "hundred-heads": dict(starts=[400, 64], S=2, h=100, R=512, rope=64, page=64, counts=[2, 1]),
+    "two-hundred-heads-missing": dict(starts=[130, 63], S=1, h=200, R=512, rope=64, page=16, lose=((0, 2, -1), (1, 0, 10**8), (0, 8, -3))),
+    "many-heads-long": dict(starts=[5000, 33, 1777], S=1, h=128, R=512, rope=64, page=64),
+    "many-heads-page-of-one": dict(starts=[45], S=1, h=64, R=512, rope=64, page=1),
+    "many-heads-negative-start": dict(starts=[-2, 31], S=2, h=128, R=512, rope=64, page=16),
     "small-widths": dict(starts=[90, 3], S=2, h=6, R=48, rope=16, page=16),
     "counts-missing": dict(starts=[60, 20, 0], S=4, h=16, R=512, rope=64, page=16, counts=[2, 4, 0], lose=((1, 0, -1), (0, 1, 10**7))),
 }
@@ -216,10 +222,10 @@ def refusals(device, dtype):
     }
 
 
-def not_finite_case(dtype, e4m3, device, latent=False, window=None):
+def not_finite_case(dtype, e4m3, device, latent=False, window=None, heads=8):
     """A draft whose third token has a NaN key, an infinite value and a NaN value in some places: earlier queries (and, with a
     window, later ones that no longer see it) must not notice.  e4m3 rows hold a NaN scale instead."""
-    c = dict(starts=[20, 70], S=5, hq=8, hkv=1 if latent else 2, page=16)
+    c = dict(starts=[20, 70], S=5, hq=heads, hkv=1 if latent else 2, page=16)
     D, R = (576, 512) if latent else (64, None)
     su = set_up(c, dtype, e4m3, device, values=not latent, d=D)
     for b in range(2):
@@ -235,11 +241,11 @@ def not_finite_case(dtype, e4m3, device, latent=False, window=None):
                 su.k_pages[pid, 1, off, 5] = float("nan")
     scale = 0.1
     if latent:
-        q, q_pe = su.normal(2, 5, 8, R), su.normal(2, 5, 8, D - R)
+        q, q_pe = su.normal(2, 5, heads, R), su.normal(2, 5, heads, D - R)
         got = ops.paged_latent_attention(q, q_pe, su.k_pages, su.table, su.starts, None, su.k_scale, scale)
         want, tol = po.attention(su, torch.cat((q, q_pe), -1), scale, latent=R, p_type=p_type(dtype, e4m3))
     else:
-        q = su.normal(2, 5, 8, D)
+        q = su.normal(2, 5, heads, D)
         got = ops.paged_attention(q, su.k_pages, su.v_pages, su.table, su.starts, None, su.k_scale, su.v_scale, scale, window)
         want, tol = po.attention(su, q, scale, window, p_type=p_type(dtype, e4m3))
     assert torch.isfinite(want[:, :2]).all() and not torch.isfinite(want[:, 2]).all()

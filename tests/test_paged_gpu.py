@@ -67,9 +67,10 @@ def test_hidden_values_that_are_not_finite(dtype, e4m3, window):
     pc.not_finite_case(dtype, e4m3, "cuda", window=window)
 
 
+@pytest.mark.parametrize("heads", [8, 64])
 @pytest.mark.parametrize("dtype,e4m3", TYPES, ids=str)
-def test_hidden_latents_that_are_not_finite(dtype, e4m3):
-    pc.not_finite_case(dtype, e4m3, "cuda", latent=True)
+def test_hidden_latents_that_are_not_finite(dtype, e4m3, heads):
+    pc.not_finite_case(dtype, e4m3, "cuda", latent=True, heads=heads)
 
 
 @pytest.mark.parametrize("shape", [(0, 1, 4, 2), (2, 0, 4, 2), (2, 1, 0, 2)])
