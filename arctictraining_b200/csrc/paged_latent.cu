@@ -523,8 +523,9 @@ constexpr int kSub = kKeys * 128;                       // 64 columns of a stage
 constexpr int kStage = kJoint / 64 * kSub;
 constexpr int kQTmem = 384, kQSub = kRows * 128;        // query columns in tensor memory; 64 columns of the others
 constexpr int kQ = 0, kK = (kJoint - kQTmem) / 64 * kQSub, kScale = kK + kRing * kStage, kValid = kScale + kRing * kKeys * 4;
-constexpr int kBars = kValid + kRing * 4 + 8, kSmem = kBars + 32 * 8 + 64;
-static_assert(kBars % 8 == 0 && kK % 1024 == 0, "aligned");
+constexpr int kBars = kValid + kRing * 4 + 8, kSmem0 = kBars + 32 * 8 + 64;
+constexpr int kSpare = (kSmem0 + 1023) / 1024 * 1024, kSmem = kSpare + 2 * kQSub;  // two more buffers of 64 query columns
+static_assert(kBars % 8 == 0 && kK % 1024 == 0 && kQTmem == 6 * 64 && kJoint == 9 * 64, "aligned, and parts as the queries are fetched");
 constexpr uint32_t kS = 256, kQCol = 320;               // columns of tensor memory: values 0, scores 256 and 288, queries 320
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kGrow = 8.f;
@@ -572,7 +573,7 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
     int* scratch = reinterpret_cast<int*>(smem + kBars + 32 * 8);  // no static memory: the tiles' alignment
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBars);
     uint64_t *k_full = bars, *k_empty = bars + kRing, *s_full = bars + 2 * kRing, *p_full = s_full + 2, *pv_done = p_full + 2,
-             *q_full = pv_done + 2;
+             *q_full = pv_done + 2, *q_sync = q_full + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* s_scale = reinterpret_cast<float*>(smem + kScale);
@@ -602,6 +603,7 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
             ptx::mbar_init(&pv_done[i], 1);
         }
         ptx::mbar_init(q_full, 128);
+        ptx::mbar_init(q_sync, 128);
         *abort_flag = 0;
         ptx::fence_barrier_init();
         ptx::fence_proxy_async_smem();
@@ -651,9 +653,8 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
             if (++t_in < p.n) look_up();
             else if ((more = walk.next(a, p))) begin_piece();
         };
-        auto place = [&](int st, int col) {  // of 16 bytes (8 elements) of this row
-            return smem + kK + st * kStage + (col >> 6) * kSub + key * 128 + ((((col >> 3) & 7) ^ (key & 7)) << 4);
-        };
+        // place in a stage of this row's 16-byte chunk 4 i + part: i even or odd, and (i / 2) kSub on
+        const int row_at[2] = {key * 128 + ((part ^ (key & 7)) << 4), key * 128 + (((part + 4) ^ (key & 7)) << 4)};
         auto mark = [&](int st, bool here) {  // the tile's keys that exist
             const uint32_t bits = __ballot_sync(0xffffffffu, here);
             if (lane == 0) {
@@ -665,30 +666,43 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
         };
         int T = 0;
         if constexpr (!E4M3) {
-            constexpr int kLag = 2;  // tiles whose copies are on their way
+            // Two tiles' copies stay on their way while the next is fetched; where the ring is full they are handed over before
+            // the wait for a stage.
+            constexpr int kLag = 2;
+            int sent = 0;
+            auto hand_over = [&](int upto) {
+                ptx::fence_proxy_async_smem();
+                for (; sent < upto; ++sent) ptx::mbar_arrive(&k_full[sent % kRing]);
+            };
+            const uint32_t stages = ptx::smem_u32(smem + kK);
             for (; more && ok; ++T) {
                 next_tile();
                 const int st = T % kRing;
-                ok = ptx::mbar_wait_bounded(&k_empty[st], ((T / kRing) & 1) ^ 1u, abort_flag, kWaitNs);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(&k_empty[st], ((T / kRing) & 1) ^ 1u))) {
+                    copies_wait<0>();
+                    hand_over(T);
+                    ok = ptx::mbar_wait_bounded(&k_empty[st], ((T / kRing) & 1) ^ 1u, abort_flag, kWaitNs);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
                 mark(st, full);
+                const uint32_t to[2] = {stages + st * kStage + row_at[0], stages + st * kStage + row_at[1]};
+                const uint8_t* from = full ? src + part * 16 : (const uint8_t*)a.k_pages;
+                if (full) {
 #pragma unroll
-                for (int i = 0; i < kJoint / 32; ++i) {
-                    const int col = (i * 4 + part) * 8;
-                    copy16(ptx::smem_u32(place(st, col)), full ? src + col * 2 : (const uint8_t*)a.k_pages, full);
+                    for (int i = 0; i < kJoint / 32; ++i) copy16(to[i & 1] + (i >> 1) * kSub, from + i * 64, true);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kJoint / 32; ++i) copy16(to[i & 1] + (i >> 1) * kSub, from, false);
                 }
                 copies_commit();
-                if (T >= kLag) {
+                if (T + 1 - sent > kLag) {
                     copies_wait<kLag>();
-                    ptx::fence_proxy_async_smem();
-                    ptx::mbar_arrive(&k_full[(T - kLag) % kRing]);
+                    hand_over(T + 1 - kLag);
                 }
             }
             copies_wait<0>();
-            ptx::fence_proxy_async_smem();
-            if (ok)
-                for (int x = max(0, T - kLag); x < T; ++x) ptx::mbar_arrive(&k_full[x % kRing]);
+            if (ok) hand_over(T);
         } else {
             uint4 now[9], ahead[9];
             float scale_now = 0.f, scale_ahead = 0.f;
@@ -718,14 +732,15 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
                 if (part == 0) s_scale[st * kKeys + key] = scale_now;
 #pragma unroll
                 for (int i = 0; i < 9; ++i) {
-                    const int col = (i * 4 + part) * 16;
+                    uint8_t* sub = smem + kK + st * kStage + i * kSub + key * 128;  // 16 of the 64 columns of part i
+                    const int ch0 = part * 2;
                     uint4 lo, hi;
                     e4m3x4_to_f16x4(now[i].x, lo.x, lo.y);
                     e4m3x4_to_f16x4(now[i].y, lo.z, lo.w);
                     e4m3x4_to_f16x4(now[i].z, hi.x, hi.y);
                     e4m3x4_to_f16x4(now[i].w, hi.z, hi.w);
-                    *reinterpret_cast<uint4*>(place(st, col)) = lo;
-                    *reinterpret_cast<uint4*>(place(st, col + 8)) = hi;
+                    *reinterpret_cast<uint4*>(sub + ((ch0 ^ (key & 7)) << 4)) = lo;
+                    *reinterpret_cast<uint4*>(sub + (((ch0 + 1) ^ (key & 7)) << 4)) = hi;
                 }
                 ptx::fence_proxy_async_smem();
                 ptx::mbar_arrive(&k_full[st]);
@@ -734,21 +749,25 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
         if (!ok && lane == 0) atomicCAS(error_flag, 0, (0x31 << 8) | 1);
     } else if (warp == 8) {
         // -------------------------------------------------------------------------------- products
-        if (lane == 0) {
+        // The thread is chosen by elect.sync: the compiler then knows that one thread issues, and a product of 32 columns takes
+        // its 16 cycles (45 to 80 behind a test of the lane, which moves every operand to uniform registers one by one).
+        if (ptx::elect_one()) {
             constexpr uint32_t fmt = std::is_same<P, bf16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t kind = ~((1u << 7) | (1u << 10));
             constexpr uint32_t idesc_qk = (ptx::make_idesc_bf16(kRows, kKeys, false, false) & kind) | fmt;
             constexpr uint32_t idesc_pv = (ptx::make_idesc_bf16(kRows, kCols, false, true) & kind) | fmt;
-            const uint32_t qs = ptx::smem_u32(smem + kQ), ks0 = ptx::smem_u32(smem + kK);
+            const uint64_t q_desc = ptx::make_smem_desc_sw128(ptx::smem_u32(smem + kQ), 16, 1024);
+            const uint64_t k_desc = ptx::make_smem_desc_sw128(ptx::smem_u32(smem + kK), 16, 1024);
+            const uint64_t v_desc = ptx::make_smem_desc_sw128(ptx::smem_u32(smem + kK), kSub, 1024);
             int T = 0, np = 0;
             bool ok = true;
             auto issue_values = [&](int t, bool add, int half) -> bool {
                 if (!ptx::mbar_wait_bounded(&p_full[t & 1], (t >> 1) & 1, abort_flag, kWaitNs)) return false;
                 ptx::tc_fence_after();
-                const uint32_t vs = ks0 + (t % kRing) * kStage + half * (kCols / 64) * kSub;
+                const uint64_t vs = v_desc + (((t % kRing) * kStage + half * (kCols / 64) * kSub) >> 4);
 #pragma unroll
                 for (int k = 0; k < kKeys / 16; ++k)
-                    ptx::mma_bf16_ts(tmem, tmem + kS + (t & 1) * kKeys + k * 8, ptx::make_smem_desc_sw128(vs + k * 2048, kSub, 1024), idesc_pv,
+                    ptx::mma_bf16_ts(tmem, tmem + kS + (t & 1) * kKeys + k * 8, vs + (k * 2048 >> 4), idesc_pv,
                                      add || k > 0);
                 ptx::mma_commit(&k_empty[t % kRing]);
                 ptx::mma_commit(&pv_done[t & 1]);
@@ -761,12 +780,13 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
                     ok = ptx::mbar_wait_bounded(&k_full[T % kRing], (T / kRing) & 1, abort_flag, kWaitNs);
                     if (!ok) break;
                     ptx::tc_fence_after();
-                    const uint32_t ks = ks0 + (T % kRing) * kStage, d = tmem + kS + (T & 1) * kKeys;
+                    const uint64_t ks = k_desc + ((T % kRing) * kStage >> 4);
+                    const uint32_t d = tmem + kS + (T & 1) * kKeys;
 #pragma unroll
                     for (int k = 0; k < kJoint / 16; ++k) {
-                        const uint64_t kd = ptx::make_smem_desc_sw128(ks + (k >> 2) * kSub + (k & 3) * 32, 16, 1024);
+                        const uint64_t kd = ks + (((k >> 2) * kSub + (k & 3) * 32) >> 4);
                         if (k < kQTmem / 16) ptx::mma_bf16_ts(d, tmem + kQCol + k * 8, kd, idesc_qk, k > 0);
-                        else ptx::mma_bf16_ss(d, ptx::make_smem_desc_sw128(qs + ((k - kQTmem / 16) >> 2) * kQSub + (k & 3) * 32, 16, 1024), kd, idesc_qk, 1u);
+                        else ptx::mma_bf16_ss(d, q_desc + ((((k - kQTmem / 16) >> 2) * kQSub + (k & 3) * 32) >> 4), kd, idesc_qk, 1u);
                     }
                     ptx::mma_commit(&s_full[T & 1]);
                     if (t > 0) ok = issue_values(T - 1, t > 1, p.half);
@@ -779,7 +799,7 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
         // -------------------------------------------------------------------------------- softmax: a query row a thread
         const int r = threadIdx.x;
         const uint32_t my = tmem + ((uint32_t)(warp * 32) << 16);
-        int T = 0;
+        int T = 0, meetings = 0;
         bool ok = true;
         // values of tile t are added: a barrier for even and one for odd tiles, since a wait names a phase by its parity only
         // and the tile before may not be done either
@@ -787,29 +807,57 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
             return (bool)__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&pv_done[t & 1], (t >> 1) & 1, abort_flag, kWaitNs));
         };
         while (ok && walk.next(a, p)) {
-            // this row's queries: [latent | rotary], zeros where the tile has no row
+            // The tile's queries [latent | rotary], zeros where it has no row: 64 columns at a time are copied to shared memory
+            // by rows (eight threads a row); each thread takes its own row from there to tensor memory, the last three
+            // parts stay.  Five parts first (two in spare buffers), then the other four.
             const bool real = r < p.rows;
-            const int gr = p.row0 + (real ? r : 0), j = p.token, h = gr - j * a.Hq;
-            const Q* ql = (const Q*)a.q + p.b * a.q_b + j * a.q_s + h * a.q_h;
-            const Q* qr = (const Q*)a.q2 + p.b * a.q2_b + j * a.q2_s + h * a.q2_h;
-            float fac = fmaxf(fabsf(a.scale), 1e-30f) * kLog2e, up = 1.f;
-            auto load_q = [&](int col) -> uint4 {
-                if (!real) return make_uint4(0, 0, 0, 0);
-                return *reinterpret_cast<const uint4*>(col < kLatent ? ql + col : qr + col - kLatent);
-            };
-            if (E4M3 && std::is_same<Q, bf16>::value) {  // the row's power of two (see the grouped form)
-                float m = 0.f;
-#pragma unroll 8
-                for (int col = 0; col < kJoint; col += 8) {
-                    const uint4 u = load_q(col);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            const int j = p.token, gr = p.row0 + r;
+            const Q* q_base = (const Q*)a.q + p.b * a.q_b + j * a.q_s + (int64_t)(p.row0 - j * a.Hq) * a.q_h;
+            const Q* q2_base = (const Q*)a.q2 + p.b * a.q2_b + j * a.q2_s + (int64_t)(p.row0 - j * a.Hq) * a.q2_h;
+            auto buffer = [&](int i) { return i < 3 ? kQ + i * kQSub : kSpare + (i - 3) * kQSub; };
+            auto fetch = [&](int part, int buf) {  // 64 columns
+                const uint32_t to = ptx::smem_u32(smem + buffer(buf));
+                const int ch = r & 7;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 y = unpack2<Q>(w[i]);
-                        m = fmaxf(m, fmaxf(fabsf(y.x), fabsf(y.y)));
-                    }
+                for (int x = 0; x < kRows / 16; ++x) {
+                    const int row = x * 16 + (r >> 3);
+                    const Q* src = part < kLatent / 64 ? q_base + row * a.q_h + part * 64 : q2_base + row * a.q2_h;
+                    const bool in = row < p.rows;
+                    copy16(to + row * 128 + ((ch ^ (row & 7)) << 4), in ? (const void*)(src + ch * 8) : a.q, in);
                 }
-                const int e = (__float_as_uint(m) >> 23) & 255;
+            };
+            auto meet = [&]() -> bool {  // the four warps, bounded
+                ptx::mbar_arrive(q_sync);
+                const bool there = ptx::mbar_wait_bounded(q_sync, meetings++ & 1, abort_flag, kWaitNs);
+                return (bool)__all_sync(0xffffffffu, there);
+            };
+            for (int part = 0; part < 5; ++part) fetch(part, part);
+            copies_commit();
+            float fac = fmaxf(fabsf(a.scale), 1e-30f) * kLog2e, up = 1.f;
+            if (E4M3 && std::is_same<Q, bf16>::value) {  // the row's power of two (see the grouped form): a warp a row, 32 rows
+                float mine = 0.f;
+#pragma unroll 4
+                for (int x = 0; x < 32; ++x) {
+                    const int row = warp * 32 + x;
+                    float m = 0.f;
+                    if (row < p.rows) {
+#pragma unroll
+                        for (int c = 0; c < 3; ++c) {
+                            const int col = (c * 32 + lane) * 8;
+                            if (col >= kJoint) continue;
+                            const uint4 u = *reinterpret_cast<const uint4*>(col < kLatent ? q_base + row * a.q_h + col : q2_base + row * a.q2_h + col - kLatent);
+                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 y = unpack2<Q>(w[i]);
+                                m = fmaxf(m, fmaxf(fabsf(y.x), fabsf(y.y)));
+                            }
+                        }
+                    }
+                    m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // magnitudes order like their bits
+                    if (lane == x) mine = m;
+                }
+                const int e = (__float_as_uint(mine) >> 23) & 255;
                 const int field = e == 0 || e == 255 ? 127 : min(268 - e, 253);
                 up = __uint_as_float((uint32_t)field << 23);
                 fac *= __uint_as_float((uint32_t)(254 - field) << 23);
@@ -823,28 +871,42 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
                 }
                 return u;
             };
-#pragma unroll 1
-            for (int c = 0; c < kQTmem / 64; ++c) {
+            auto chunk = [&](int buf, int i) { return reinterpret_cast<uint4*>(smem + buffer(buf) + r * 128 + ((i ^ (r & 7)) << 4)); };
+            auto to_tmem = [&](int part, int buf) {
                 uint32_t v[32];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint4 u = load_q(c * 64 + i * 8);
+                    const uint4 u = *chunk(buf, i);
                     v[4 * i] = turn(u.x);
                     v[4 * i + 1] = turn(u.y);
                     v[4 * i + 2] = turn(u.z);
                     v[4 * i + 3] = turn(u.w);
                 }
                 __syncwarp();
-                ptx::tmem_st_32x32b_x32(my + kQCol + c * 32, v);
-            }
-#pragma unroll 8
-            for (int i = 0; i < (kJoint - kQTmem) / 8; ++i) {
-                uint4 u = load_q(kQTmem + i * 8);
-                u.x = turn(u.x);
-                u.y = turn(u.y);
-                u.z = turn(u.z);
-                u.w = turn(u.w);
-                *reinterpret_cast<uint4*>(smem + kQ + (i >> 3) * kQSub + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = u;
+                ptx::tmem_st_32x32b_x32(my + kQCol + part * 32, v);
+            };
+            copies_wait<0>();
+            if (!(ok = meet())) break;
+#pragma unroll 1
+            for (int part = 0; part < 5; ++part) to_tmem(part, part);
+            if (!(ok = meet())) break;  // the buffers have been read
+            fetch(5, 3);
+            for (int part = 6; part < 9; ++part) fetch(part, part - 6);
+            copies_commit();
+            copies_wait<0>();
+            if (!(ok = meet())) break;
+            to_tmem(5, 3);
+            if (sign || (E4M3 && std::is_same<Q, bf16>::value)) {
+#pragma unroll 1
+                for (int x = 0; x < 24; ++x) {
+                    uint4* at = chunk(x >> 3, x & 7);
+                    uint4 u = *at;
+                    u.x = turn(u.x);
+                    u.y = turn(u.y);
+                    u.z = turn(u.z);
+                    u.w = turn(u.w);
+                    *at = u;
+                }
             }
             __syncwarp();
             ptx::tmem_st_wait();
