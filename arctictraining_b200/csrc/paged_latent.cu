@@ -5,6 +5,7 @@
 
 namespace atb {
 
+CUtensorMap make_tmap_bf16_public(const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows);
 at::Tensor& gemm_error_flag(const at::Device& dev);
 
 namespace paged {
@@ -567,7 +568,8 @@ struct Walk {
 
 template <typename Q, bool E4M3>
 __global__ void __launch_bounds__(kThreads, 1)
-latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __restrict__ part_ml, float* __restrict__ part_o, int* error_flag) {
+latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const AttnArgs a, int B, int4* __restrict__ jobs,
+                 float* __restrict__ part_ml, float* __restrict__ part_o, int* error_flag) {
     using P = typename std::conditional<E4M3, __half, Q>::type;
     extern __shared__ __align__(1024) uint8_t smem[];
     int* scratch = reinterpret_cast<int*>(smem + kBars + 32 * 8);  // no static memory: the tiles' alignment
@@ -637,9 +639,12 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
         // source of this thread's row of the next tile, which then moves on
         const uint8_t* src = nullptr;
         const float* scale_src = nullptr;
-        bool full = false;
+        bool full = false, dense = false;  // this thread's key exists; the tile is 32 rows of one page
+        int row0 = 0;
         auto next_tile = [&]() {
             full = pid >= 0 && pid < a.P;
+            dense = page_rows > 0 && full && pos - key + kKeys <= upto;
+            row0 = pid * page_rows + off - key;
             const int64_t row = full ? pid * a.k_page + (int64_t)off * kJoint : 0;
             src = (const uint8_t*)a.k_pages + row * (E4M3 ? 1 : 2);
             if (E4M3) scale_src = a.k_scale + (full ? pid * a.ks_page + off : 0);
@@ -684,6 +689,21 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
                     ok = ptx::mbar_wait_bounded(&k_empty[st], ((T / kRing) & 1) ^ 1u, abort_flag, kWaitNs);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
+                }
+                if (dense) {  // the same for all threads: one fetches the tile, nine parts of 64 columns
+                    copies_wait<0>();
+                    hand_over(T);
+                    if (tid == 0) {
+                        s_valid[st] = 0xffffffffu;
+                        ptx::mbar_expect_tx(&k_full[st], kStage);
+#pragma unroll
+                        for (int i = 0; i < kJoint / 64; ++i)
+                            ptx::tma_load_2d(smem + kK + st * kStage + i * kSub, &tmap, i * 64, row0, &k_full[st]);
+                    } else {
+                        ptx::mbar_arrive(&k_full[st]);
+                    }
+                    ++sent;
+                    continue;
                 }
                 mark(st, full);
                 const uint32_t to[2] = {stages + st * kStage + row_at[0], stages + st * kStage + row_at[1]};
@@ -836,26 +856,33 @@ latent_tc_kernel(const AttnArgs a, int B, int4* __restrict__ jobs, float* __rest
             float fac = fmaxf(fabsf(a.scale), 1e-30f) * kLog2e, up = 1.f;
             if (E4M3 && std::is_same<Q, bf16>::value) {  // the row's power of two (see the grouped form): a warp a row, 32 rows
                 float mine = 0.f;
-#pragma unroll 4
-                for (int x = 0; x < 32; ++x) {
-                    const int row = warp * 32 + x;
-                    float m = 0.f;
-                    if (row < p.rows) {
+#pragma unroll 1
+                for (int x0 = 0; x0 < 32; x0 += 8) {  // eight rows on their way at a time
+                    uint4 u[8][3];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
 #pragma unroll
                         for (int c = 0; c < 3; ++c) {
-                            const int col = (c * 32 + lane) * 8;
-                            if (col >= kJoint) continue;
-                            const uint4 u = *reinterpret_cast<const uint4*>(col < kLatent ? q_base + row * a.q_h + col : q2_base + row * a.q2_h + col - kLatent);
-                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                            const int row = warp * 32 + x0 + x, col = (c * 32 + lane) * 8;
+                            u[x][c] = make_uint4(0, 0, 0, 0);
+                            if (row < p.rows && col < kJoint)
+                                u[x][c] = *reinterpret_cast<const uint4*>(col < kLatent ? q_base + row * a.q_h + col : q2_base + row * a.q2_h + col - kLatent);
+                        }
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        float m = 0.f;
+#pragma unroll
+                        for (int c = 0; c < 3; ++c) {
+                            const uint32_t w[4] = {u[x][c].x, u[x][c].y, u[x][c].z, u[x][c].w};
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const float2 y = unpack2<Q>(w[i]);
                                 m = fmaxf(m, fmaxf(fabsf(y.x), fabsf(y.y)));
                             }
                         }
+                        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // magnitudes order like their bits
+                        if (lane == x0 + x) mine = m;
                     }
-                    m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // magnitudes order like their bits
-                    if (lane == x) mine = m;
                 }
                 const int e = (__float_as_uint(mine) >> 23) & 255;
                 const int field = e == 0 || e == 255 ? 127 : min(268 - e, 253);
@@ -1067,7 +1094,14 @@ static void launch_latent_tc(AttnArgs a, int64_t B, const at::Tensor& q) {
     const Workspace ws(q, ctas, tc::kRows, a.cols);
     cudaStream_t st = current_stream();
     int* error = gemm_error_flag(q.device()).data_ptr<int>();
-    tc::latent_tc_kernel<T, E4M3><<<ctas, tc::kThreads, tc::kSmem, st>>>(a, (int)B, ws.jobs, ws.ml, ws.o, error);
+    // whole tiles come by TMA where a tile cannot cross pages and pages lie a whole number of rows apart
+    CUtensorMap tmap = {};
+    int page_rows = 0;
+    if (!E4M3 && a.page % tc::kKeys == 0 && a.k_page % kJoint == 0 && (int64_t)a.P * (a.k_page / kJoint) < (int64_t(1) << 31)) {
+        page_rows = (int)(a.k_page / kJoint);
+        tmap = make_tmap_bf16_public(a.k_pages, (int64_t)(a.P - 1) * page_rows + a.page, kJoint, kJoint, tc::kKeys);
+    }
+    tc::latent_tc_kernel<T, E4M3><<<ctas, tc::kThreads, tc::kSmem, st>>>(tmap, page_rows, a, (int)B, ws.jobs, ws.ml, ws.o, error);
     ATB_LAUNCH_CHECK();
     launch_join<T>(a, tc::kRows, ctas, ws, st);
 }
