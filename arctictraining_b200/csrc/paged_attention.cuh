@@ -207,24 +207,17 @@ __device__ __forceinline__ bool values_not_finite(F&& load) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Adds the pieces of an item that several CTAs of the attention kernel worked on, in their order along the keys.  Such an item
-// lies across the begin of some CTA's piece; the attention kernel left a job there.  Every block gathers the jobs, all in the
-// same order, and the blocks share out (job, query row, 128 columns): a warp each where the items have few pieces, a block
-// each, its warps taking pieces in turn, where some item has many.  The kernel is launched while the attention kernel runs, and
-// waits for its end before it reads.  (Its pointers are not declared free of aliases: loads that are known to be invariant may
-// be moved ahead of the wait.)
 constexpr int kMaxCtas = 1024;
-template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int rows, int ctas, const int4* jobs, const float* part_ml,
-                                                   const float* part_o) {
-    __shared__ int4 s_jobs[kMaxCtas];
-    __shared__ int s_first[kMaxCtas], s_place[32], s_most;
-    __shared__ float2 s_ml[kMaxCtas];
-    __shared__ float s_red[2][4];
-    __shared__ float4 s_o[128];
+struct JobList {  // in shared memory
+    int4 jobs[kMaxCtas];
+    int first[kMaxCtas], place[32], most;  // the CTA that began the item; most pieces of one
+};
+// All blocks of a joining kernel (128 threads) wait for the attention kernel, launched before, and gather its jobs in the
+// order of their CTAs.  Returns their number.  (The pointers of such kernels are not declared free of aliases: loads that are
+// known to be invariant may be moved ahead of the wait.)
+__device__ __forceinline__ int gather_jobs(JobList& list, int ctas, const int4* jobs) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int G = a.Hq / a.Hkv, M = a.S * G;
-    if (threadIdx.x == 0) s_most = 0;
+    if (threadIdx.x == 0) list.most = 0;
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int4 mine[kMaxCtas / 128];
@@ -238,10 +231,10 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int rows, i
 #pragma unroll
     for (int x = 0; x < kMaxCtas / 128; ++x) {
         has[x] = __ballot_sync(0xffffffffu, mine[x].z > 0);
-        if (lane == 0) s_place[x * 4 + warp] = __popc(has[x]);
+        if (lane == 0) list.place[x * 4 + warp] = __popc(has[x]);
     }
     __syncthreads();
-    int upto = s_place[lane];
+    int upto = list.place[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -253,20 +246,37 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int rows, i
         const int base = __shfl_sync(0xffffffffu, upto, x * 4 + warp) - __popc(has[x]);
         if (mine[x].z > 0) {
             const int at = base + __popc(has[x] & ((1u << lane) - 1));
-            s_jobs[at] = mine[x];
-            s_first[at] = threadIdx.x + 128 * x - 1;
-            atomicMax(&s_most, mine[x].z);
+            list.jobs[at] = mine[x];
+            list.first[at] = threadIdx.x + 128 * x - 1;
+            atomicMax(&list.most, mine[x].z);
         }
     }
     __syncthreads();
+    return n_jobs;
+}
+
+// Adds the pieces of an item that several CTAs of the attention kernel worked on, in their order along the keys.  Such an item
+// lies across the begin of some CTA's piece; the attention kernel left a job there.  Every block gathers the jobs, all in the
+// same order, and the blocks share out (job, query row, 128 columns): a warp each where the items have few pieces, a block
+// each, its warps taking pieces in turn, where some item has many.
+template <typename T>
+__global__ void __launch_bounds__(128) join_kernel(const AttnArgs a, int rows, int ctas, const int4* jobs, const float* part_ml,
+                                                   const float* part_o) {
+    __shared__ JobList list;
+    __shared__ float2 s_ml[kMaxCtas];
+    __shared__ float s_red[2][4];
+    __shared__ float4 s_o[128];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n_jobs = gather_jobs(list, ctas, jobs);
+    const int G = a.Hq / a.Hkv, M = a.S * G;
     const int used = min(rows, a.token_tiles ? G : M), slices = (a.cols / 4 + 31) / 32;
     const int total = n_jobs * used * slices;
-    const bool wide = s_most > 8;  // a block for each unit
+    const bool wide = list.most > 8;  // a block for each unit
     for (int u = wide ? blockIdx.x : blockIdx.x * 4 + warp; u < total; u += wide ? gridDim.x : gridDim.x * 4) {
         const int col = (u % slices) * 128 + lane * 4, rest = u / slices;
         const int r = rest % used, jb = rest / used;
-        const int4 job = s_jobs[jb];
-        const int b = job.x, n = job.z, cta = s_first[jb];
+        const int4 job = list.jobs[jb];
+        const int b = job.x, n = job.z, cta = list.first[jb];
         int h, half, row0, real;
         item_rows(a, job.y, rows, h, half, row0, real);
         if (r >= real) continue;
@@ -372,10 +382,11 @@ struct Workspace {
     }
 };
 
-template <typename T>
-static void launch_join(const AttnArgs& a, int rows, int ctas, const Workspace& ws, cudaStream_t st) {
+// Launches a joining kernel (`per_sm` blocks an SM) that may be set up while the attention kernel before it runs.
+template <typename... P, typename... X>
+static void launch_behind(void (*kernel)(P...), int per_sm, cudaStream_t st, X... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)at::cuda::getCurrentDeviceProperties()->multiProcessorCount * 4);
+    cfg.gridDim = dim3((unsigned)(at::cuda::getCurrentDeviceProperties()->multiProcessorCount * per_sm));
     cfg.blockDim = dim3(128);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -383,7 +394,11 @@ static void launch_join(const AttnArgs& a, int rows, int ctas, const Workspace& 
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T>, a, rows, ctas, (const int4*)ws.jobs, (const float*)ws.ml, (const float*)ws.o));
+    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+template <typename T>
+static void launch_join(const AttnArgs& a, int rows, int ctas, const Workspace& ws, cudaStream_t st) {
+    launch_behind(join_kernel<T>, 4, st, a, rows, ctas, (const int4*)ws.jobs, (const float*)ws.ml, (const float*)ws.o);
 }
 
 inline bool half_type(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }

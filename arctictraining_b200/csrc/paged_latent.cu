@@ -523,7 +523,7 @@ constexpr int kThreads = 288, kKeys = 32, kRing = 4, kRows = 128, kCols = 256;
 constexpr int kSub = kKeys * 128;                       // 64 columns of a stage, 128-byte swizzled rows
 constexpr int kStage = kJoint / 64 * kSub;
 constexpr int kQTmem = 384, kQSub = kRows * 128;        // query columns in tensor memory; 64 columns of the others
-constexpr int kQ = 0, kK = (kJoint - kQTmem) / 64 * kQSub, kScale = kK + kRing * kStage, kValid = kScale + kRing * kKeys * 4;
+constexpr int kQ = 0, kK = (kJoint - kQTmem) / 64 * kQSub, kScale = kK + kRing * kStage, kValid = kScale + 2 * kRing * kKeys * 4;
 constexpr int kBars = kValid + kRing * 4 + 8, kSmem0 = kBars + 32 * 8 + 64;
 constexpr int kSpare = (kSmem0 + 1023) / 1024 * 1024, kSmem = kSpare + 2 * kQSub;  // two more buffers of 64 query columns
 static_assert(kBars % 8 == 0 && kK % 1024 == 0 && kQTmem == 6 * 64 && kJoint == 9 * 64, "aligned, and parts as the queries are fetched");
@@ -749,7 +749,10 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 mark(st, here);
-                if (part == 0) s_scale[st * kKeys + key] = scale_now;
+                if (part == 0) {  // the scale, and its logarithm
+                    s_scale[st * kKeys + key] = scale_now;
+                    s_scale[(kRing + st) * kKeys + key] = __log2f(scale_now);
+                }
 #pragma unroll
                 for (int i = 0; i < 9; ++i) {
                     uint8_t* sub = smem + kK + st * kStage + i * kSub + key * 128;  // 16 of the 64 columns of part i
@@ -964,10 +967,11 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
                         x[i + 1] *= sc.y;
                         x[i + 2] *= sc.z;
                         x[i + 3] *= sc.w;
-                        lv[i] = __log2f(sc.x);
-                        lv[i + 1] = __log2f(sc.y);
-                        lv[i + 2] = __log2f(sc.z);
-                        lv[i + 3] = __log2f(sc.w);
+                        const float4 lg = *reinterpret_cast<const float4*>(s_scale + (kRing + st) * kKeys + i);
+                        lv[i] = lg.x;
+                        lv[i + 1] = lg.y;
+                        lv[i + 2] = lg.z;
+                        lv[i + 3] = lg.w;
                     }
                 }
                 if (valid != 0xffffffffu) {
@@ -1036,7 +1040,8 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
             // a whole item is divided by its sum; a piece's values are brought to the units of its sum, 2^m
             float f = E4M3 ? (mv == -INFINITY ? 0.f : exp2f(mv - m)) : 1.f;
             if (p.whole) f = __fdividef(f, l);
-            const int64_t part = ((int64_t)blockIdx.x * 2 + (p.first ? 0 : 1)) * kRows + r;
+            // pieces lie in groups of four columns, [column / 4][row][4]: a warp's 32 rows are one dense store
+            const int64_t part0 = ((int64_t)blockIdx.x * 2 + (p.first ? 0 : 1)) * kRows;
             Q* out = (Q*)a.out + ((int64_t)p.b * a.S * a.Hq + gr) * kLatent + p.half * kCols;
 #pragma unroll 1
             for (int c = 0; c < kCols; c += 32) {
@@ -1056,14 +1061,14 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4*>(part_o + part * kCols + c + i) =
+                        *reinterpret_cast<float4*>(part_o + part0 * kCols + ((c + i) / 4 * kRows + r) * 4) =
                             make_float4(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f, __uint_as_float(v[i + 2]) * f,
                                         __uint_as_float(v[i + 3]) * f);
                 }
             }
             if (!p.whole && real) {
-                part_ml[part * 2] = m;
-                part_ml[part * 2 + 1] = l;
+                part_ml[(part0 + r) * 2] = m;
+                part_ml[(part0 + r) * 2 + 1] = l;
             }
             ptx::tc_fence_before();
         }
@@ -1077,6 +1082,78 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
         ptx::tmem_dealloc(tmem, 512);
     }
 }
+// Adds the pieces of an item, in their order along the keys: a lane a row, 8 groups of four columns.  One warp takes a
+// unit of 32 rows and 32 columns, or, where some item has many pieces, a block whose warps take pieces in turn.
+template <typename T>
+__global__ void __launch_bounds__(128) join_tiles_kernel(const AttnArgs a, int ctas, const int4* jobs, const float* part_ml,
+                                                         const float* part_o) {
+    __shared__ JobList list;
+    __shared__ float4 s_o[3][8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n_jobs = gather_jobs(list, ctas, jobs);
+    constexpr int kRowUnits = kRows / 32, kColUnits = kCols / 32;
+    const bool wide = list.most > 8;
+    for (int u = wide ? blockIdx.x : blockIdx.x * 4 + warp; u < n_jobs * kRowUnits * kColUnits; u += wide ? gridDim.x : gridDim.x * 4) {
+        const int jb = u / (kRowUnits * kColUnits), r = u / kColUnits % kRowUnits * 32 + lane, col = u % kColUnits * 32;
+        const int4 job = list.jobs[jb];
+        int h, half, row0, rows;
+        item_rows(a, job.y, kRows, h, half, row0, rows);
+        auto place = [&](int i) { return ((int64_t)(list.first[jb] + i) * 2 + (i == 0 ? job.w : 0)) * kRows; };
+        auto ml = [&](int i) { return r < rows ? *reinterpret_cast<const float2*>(part_ml + (place(i) + r) * 2) : make_float2(-INFINITY, 0.f); };
+        float top = -INFINITY, sum = 0.f;
+        for (int i = 0; i < job.z; ++i) top = fmaxf(top, ml(i).x);
+        float4 v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = wide ? warp : 0; i < job.z; i += wide ? 4 : 1) {
+            const float w = ml(i).x == -INFINITY ? 0.f : exp2f(ml(i).x - top);
+            const float4* src = reinterpret_cast<const float4*>(part_o + place(i) * kCols) + col / 4 * kRows + r;
+            if (r < rows)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const float4 o = src[c * kRows];
+                    v[c].x += o.x * w;
+                    v[c].y += o.y * w;
+                    v[c].z += o.z * w;
+                    v[c].w += o.w * w;
+                }
+        }
+        for (int i = 0; i < job.z; ++i) {  // a piece without a finite score has seen nothing, or a NaN that its sum holds
+            const float2 x = ml(i);
+            sum += x.x == -INFINITY ? x.y : x.y * exp2f(x.x - top);
+        }
+        if (wide) {
+            __syncthreads();  // the unit before has been read
+            if (warp > 0)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) s_o[warp - 1][c][lane] = v[c];
+            __syncthreads();
+            if (warp > 0) continue;
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const float4 o = s_o[x][c][lane];
+                    v[c].x += o.x;
+                    v[c].y += o.y;
+                    v[c].z += o.z;
+                    v[c].w += o.w;
+                }
+        }
+        if (r >= rows) continue;
+        const int gr = row0 + r, count = a.counts ? max(0, min(a.counts[job.x], a.S)) : a.S;
+        const bool none = gr / a.Hq >= count || sum == 0.f;
+        const float inv = __fdividef(1.f, sum);
+        T* out = (T*)a.out + ((int64_t)job.x * a.S * a.Hq + gr) * kLatent + half * kCols + col;
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) {
+            float e[8] = {v[c].x, v[c].y, v[c].z, v[c].w, v[c + 1].x, v[c + 1].y, v[c + 1].z, v[c + 1].w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = none ? 0.f : e[k] * inv;
+            *reinterpret_cast<uint4*>(out + c * 4) = Vec8<T>::pack(e);
+        }
+    }
+}
 }  // namespace tc
 
 template <typename T, bool E4M3>
@@ -1087,7 +1164,7 @@ static void launch_latent_tc(AttnArgs a, int64_t B, const at::Tensor& q) {
     a.halves = 2;
     a.cols = tc::kCols;
     a.token_tiles = (a.Hq + tc::kRows - 1) / tc::kRows;
-    a.lead = 8;
+    a.lead = 14;  // what an item costs besides its keys: queries 3 us, first keys 1.5 us, result 3 us; a round 0.6 us
     const int64_t items = (int64_t)a.S * a.token_tiles * a.halves;
     ATB_ARG(B * items * (ceil_div((int64_t)a.W * a.page, tc::kKeys) + 1 + a.lead) < (int64_t(1) << 31),
             "paged_latent_attention: too many sequences, query rows or positions for one call");
@@ -1103,7 +1180,7 @@ static void launch_latent_tc(AttnArgs a, int64_t B, const at::Tensor& q) {
     }
     tc::latent_tc_kernel<T, E4M3><<<ctas, tc::kThreads, tc::kSmem, st>>>(tmap, page_rows, a, (int)B, ws.jobs, ws.ml, ws.o, error);
     ATB_LAUNCH_CHECK();
-    launch_join<T>(a, tc::kRows, ctas, ws, st);
+    launch_behind(tc::join_tiles_kernel<T>, 4, st, a, ctas, (const int4*)ws.jobs, (const float*)ws.ml, (const float*)ws.o);
 }
 
 template <typename T, bool E4M3>
