@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, int4
             row[i] = row_base + g + 8 * i;
             const int j = min(row[i], M - 1) / G;
             hi[i] = (int)min((int64_t)rg.start + j, (int64_t)rg.total - 1);
-            lo[i] = a.window > 0 ? (int)max((int64_t)0, (int64_t)rg.start + j + 1 - a.window) : 0;
+            lo[i] = a.window > 0 ? (int)min((int64_t)rg.total, max((int64_t)0, (int64_t)rg.start + j + 1 - a.window)) : 0;
             const T* src = (const T*)a.q + b * a.q_b + (int64_t)j * a.q_s + (int64_t)(h * G + min(row[i], M - 1) % G) * a.q_h;
             const bool real = row[i] < M;
 #pragma unroll
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const AttnArgs a, int B, int4
                     const int last = min(row_base + 15, M - 1) / G;
                     for (int j = row_base / G; j <= last; ++j) {
                         const int hj = (int)min((int64_t)rg.start + j, (int64_t)rg.total - 1);
-                        const int lj = a.window > 0 ? (int)max((int64_t)0, (int64_t)rg.start + j + 1 - a.window) : 0;
+                        const int lj = a.window > 0 ? (int)min((int64_t)rg.total, max((int64_t)0, (int64_t)rg.start + j + 1 - a.window)) : 0;
 #pragma unroll 1
                         for (int kp = 0; kp < KB / 16; ++kp) {
                             uint32_t keep[2];

@@ -1082,63 +1082,68 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
         ptx::tmem_dealloc(tmem, 512);
     }
 }
-// Adds the pieces of an item, in their order along the keys: a lane a row, 8 groups of four columns.  One warp takes a
-// unit of 32 rows and 32 columns, or, where some item has many pieces, a block whose warps take pieces in turn.
+// Adds the pieces of an item, in their order along the keys: a lane a row.  One warp takes 32 rows and 32 columns or, where
+// some item has many pieces, a block takes 32 rows and 8 columns and its warps every fourth piece.
 template <typename T>
 __global__ void __launch_bounds__(128) join_tiles_kernel(const AttnArgs a, int ctas, const int4* jobs, const float* part_ml,
                                                          const float* part_o) {
     __shared__ JobList list;
-    __shared__ float4 s_o[3][8][32];
+    __shared__ float4 s_o[4][2][32];
+    __shared__ float2 s_ml[4][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n_jobs = gather_jobs(list, ctas, jobs);
-    constexpr int kRowUnits = kRows / 32, kColUnits = kCols / 32;
     const bool wide = list.most > 8;
-    for (int u = wide ? blockIdx.x : blockIdx.x * 4 + warp; u < n_jobs * kRowUnits * kColUnits; u += wide ? gridDim.x : gridDim.x * 4) {
-        const int jb = u / (kRowUnits * kColUnits), r = u / kColUnits % kRowUnits * 32 + lane, col = u % kColUnits * 32;
+    const int quads = wide ? 2 : 8, col_units = kCols / 4 / quads;
+    constexpr int kRowUnits = kRows / 32;
+    for (int u = wide ? blockIdx.x : blockIdx.x * 4 + warp; u < n_jobs * kRowUnits * col_units; u += wide ? gridDim.x : gridDim.x * 4) {
+        const int jb = u / (kRowUnits * col_units), r = u / col_units % kRowUnits * 32 + lane, col = u % col_units * quads * 4;
         const int4 job = list.jobs[jb];
         int h, half, row0, rows;
         item_rows(a, job.y, kRows, h, half, row0, rows);
-        auto place = [&](int i) { return ((int64_t)(list.first[jb] + i) * 2 + (i == 0 ? job.w : 0)) * kRows; };
-        auto ml = [&](int i) { return r < rows ? *reinterpret_cast<const float2*>(part_ml + (place(i) + r) * 2) : make_float2(-INFINITY, 0.f); };
         float top = -INFINITY, sum = 0.f;
-        for (int i = 0; i < job.z; ++i) top = fmaxf(top, ml(i).x);
         float4 v[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = wide ? warp : 0; i < job.z; i += wide ? 4 : 1) {
-            const float w = ml(i).x == -INFINITY ? 0.f : exp2f(ml(i).x - top);
-            const float4* src = reinterpret_cast<const float4*>(part_o + place(i) * kCols) + col / 4 * kRows + r;
-            if (r < rows)
+        // adds (m, l, values in units of 2^m); a piece without a finite score has seen nothing, or a NaN that its sum holds
+        auto add = [&](float m, float l, const float4 (&o)[8]) {
+            const float mn = fmaxf(top, m);
+            const float f0 = top == -INFINITY ? 0.f : exp2f(top - mn), f1 = m == -INFINITY ? 0.f : exp2f(m - mn);
+            sum = (top == -INFINITY ? sum : sum * f0) + (m == -INFINITY ? l : l * f1);
+            top = mn;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float4 o = src[c * kRows];
-                    v[c].x += o.x * w;
-                    v[c].y += o.y * w;
-                    v[c].z += o.z * w;
-                    v[c].w += o.w * w;
-                }
-        }
-        for (int i = 0; i < job.z; ++i) {  // a piece without a finite score has seen nothing, or a NaN that its sum holds
-            const float2 x = ml(i);
-            sum += x.x == -INFINITY ? x.y : x.y * exp2f(x.x - top);
+            for (int c = 0; c < 8; ++c) {
+                v[c].x = v[c].x * f0 + o[c].x * f1;
+                v[c].y = v[c].y * f0 + o[c].y * f1;
+                v[c].z = v[c].z * f0 + o[c].z * f1;
+                v[c].w = v[c].w * f0 + o[c].w * f1;
+            }
+        };
+        if (r < rows) {
+#pragma unroll 2
+            for (int i = wide ? warp : 0; i < job.z; i += wide ? 4 : 1) {
+                const int64_t at = ((int64_t)(list.first[jb] + i) * 2 + (i == 0 ? job.w : 0)) * kRows;
+                const float2 ml = *reinterpret_cast<const float2*>(part_ml + (at + r) * 2);
+                const float4* src = reinterpret_cast<const float4*>(part_o + at * kCols) + col / 4 * kRows + r;
+                float4 o[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) o[c] = c < quads ? src[c * kRows] : make_float4(0.f, 0.f, 0.f, 0.f);
+                add(ml.x, ml.y, o);
+            }
         }
         if (wide) {
             __syncthreads();  // the unit before has been read
-            if (warp > 0)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) s_o[warp - 1][c][lane] = v[c];
+            s_ml[warp][lane] = make_float2(top, sum);
+            s_o[warp][0][lane] = v[0];
+            s_o[warp][1][lane] = v[1];
             __syncthreads();
             if (warp > 0) continue;
 #pragma unroll
-            for (int x = 0; x < 3; ++x)
+            for (int x = 1; x < 4; ++x) {
+                float4 o[8];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float4 o = s_o[x][c][lane];
-                    v[c].x += o.x;
-                    v[c].y += o.y;
-                    v[c].z += o.z;
-                    v[c].w += o.w;
-                }
+                for (int c = 0; c < 8; ++c) o[c] = c < 2 ? s_o[x][c][lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+                add(s_ml[x][lane].x, s_ml[x][lane].y, o);
+            }
         }
         if (r >= rows) continue;
         const int gr = row0 + r, count = a.counts ? max(0, min(a.counts[job.x], a.S)) : a.S;
@@ -1147,6 +1152,7 @@ __global__ void __launch_bounds__(128) join_tiles_kernel(const AttnArgs a, int c
         T* out = (T*)a.out + ((int64_t)job.x * a.S * a.Hq + gr) * kLatent + half * kCols + col;
 #pragma unroll
         for (int c = 0; c < 8; c += 2) {
+            if (c >= quads) break;
             float e[8] = {v[c].x, v[c].y, v[c].z, v[c].w, v[c + 1].x, v[c + 1].y, v[c + 1].z, v[c + 1].w};
 #pragma unroll
             for (int k = 0; k < 8; ++k) e[k] = none ? 0.f : e[k] * inv;
@@ -1185,8 +1191,9 @@ static void launch_latent_tc(AttnArgs a, int64_t B, const at::Tensor& q) {
 
 template <typename T, bool E4M3>
 static void launch_latent(const AttnArgs& a, int64_t B, const at::Tensor& q) {
-    // MEASURE
-    if (a.Hq >= 64 && a.D1 == kLatent && a.D == kJoint) return launch_latent_tc<T, E4M3>(a, B, q);
+    // The tensor-core form from 33 heads on, where the other needs a second tile of 32 rows a token and with it the keys a
+    // second time (89585 positions: 32 heads 46 us in one tile; 48 heads 78 us in two and 55 us here, 64 heads 80 and 56 us).  Several tokens of few heads stay with the other: here each token has tiles of its own.
+    if (a.Hq > 32 && a.D1 == kLatent && a.D == kJoint) return launch_latent_tc<T, E4M3>(a, B, q);
     if (a.S * a.Hq <= 16) launch_latent_rows<T, E4M3, 1>(a, B, q);
     else launch_latent_rows<T, E4M3, 2>(a, B, q);
 }
