@@ -52,8 +52,9 @@ __device__ __forceinline__ void item_rows(const AttnArgs& a, int item, int rows,
 // ---- schedule ---------------------------------------------------------------------------------------------------------
 // Work is counted in rounds of `NK` keys of one item (sequence, cache head, tile of query rows).  The rounds of all items
 // stand in one line, each item's behind `lead` empty ones that stand for what an item costs besides its keys (its queries,
-// the pipeline's filling, the result: 2 to 3 us, a round 1.5 to 2 us), and every CTA takes an equal piece of the line, so a batch of very different lengths loads all SMs alike
-// and a single long sequence is spread over all of them.  A CTA that covers an item alone writes the result; otherwise it
+// the pipeline's filling, the result: 2 to 3 us for grouped heads, where a round takes 1.5 to 2 us), and every CTA takes an
+// equal piece of the line, so a batch of very different lengths loads all SMs alike and a single long sequence is spread over
+// all of them (without the empty rounds the ragged batch below took 88 us, 15 of them for the CTA with most items).  A CTA that covers an item alone writes the result; otherwise it
 // leaves (maximum, sum, weighted values) of its piece in the workspace, and the join kernel adds the pieces in their
 // order.  No atomics: the same inputs give the same bits.
 struct Range {  // the cached positions that the queries of one sequence see

@@ -17,6 +17,9 @@ namespace paged {
 // steps of 16 are divided over four groups of warps (whose slice of the queries stays in registers) and the keys over two, so
 // every key byte is read from shared memory once; the four partial sums meet in shared memory, where the softmax is taken by
 // all threads.  Weighted values: every warp reads its own 64 columns of the same tile.  Precision is that of the grouped form.
+// Measured with 16 heads: one sequence of 4003 positions 15 us; 89585 positions in 32 sequences (106 MB) 34 us, 48 % of a plain
+// copy's rate (a tile of 64 keys takes 2 us, 1.75 of them its 74 KB; ten tiles a CTA do not hide the 7 us of an item's begin and
+// end and the joining); 32 heads 46 us.
 constexpr int kLatent = 512, kRotary = 64, kJoint = kLatent + kRotary;
 
 template <bool E4M3, int MT>
@@ -518,6 +521,9 @@ static void launch_latent_rows(AttnArgs a, int64_t B, const at::Tensor& q) {
 // (8-bit ones are turned into fp16 on the way).  Warp 8 issues the products; scores of the next tile run ahead of the values
 // of this one.  All keys that a row tile sees are the same for its rows (one token), so hidden keys are never fetched.
 // The accumulator is rescaled only when a row's maximum grew by more than 2^8.  All waits are bounded.
+// Measured: 128 heads, 89585 positions in 32 sequences (25 GFLOP, 112 MB) 59 us: the products take 24 of them (1070 cycles a
+// tile of 32 keys, as the instruction rates say), queries, first keys, results and the joining of a CTA's two or three pieces
+// the rest; 8-bit 75 us (softmax with two exponentials a score); one sequence of 60000 positions 45 us.
 namespace tc {
 constexpr int kThreads = 288, kKeys = 32, kRing = 4, kRows = 128, kCols = 256;
 constexpr int kSub = kKeys * 128;                       // 64 columns of a stage, 128-byte swizzled rows

@@ -153,7 +153,7 @@ class MLAttention(nn.Module):
         q_nope = q[..., : kv.nope]
         norm = kv.kv_a_layernorm
         q_pe = cache.append_latent(self.layer_idx, q[..., kv.nope :], kv.kv_a_proj_with_mqa(x), norm.weight, norm.eps, ctx.cos, ctx.sin)
-        if S <= cache.draft_tokens and type(kv.kv_b_proj) is Linear:
+        if cache.on_pages(S) and type(kv.kv_b_proj) is Linear:
             w = kv.kv_b_proj.weight.view(H, kv.nope + kv.vd, kv.rank)
             q_latent = torch.einsum("bshn,hnr->bshr", q_nope, w[:, : kv.nope])
             latent = cache.attend_latent(self.layer_idx, q_latent, q_pe, self.scale)

@@ -4,14 +4,17 @@
 A cache is ``pages [P, heads, page, dim]``: page ``p`` holds ``page`` consecutive positions of one sequence.  Its elements
 have the model's type, or are e4m3 with one fp32 scale per position and head (``[P, heads, page]``).  ``page_table [B, W]``
 (int32) names the pages of every sequence in order; an id outside ``[0, P)`` stands for no page: writes to it are dropped and
-reads skip it.  ``starts [B]`` (int32) are the tokens that a sequence had before the call; its new token ``j`` stands at
+reads skip it.  The heads, positions and elements of a page are dense; pages may lie further apart (slices of a larger tensor),
+keys and values equally far.  ``starts [B]`` (int32) are the tokens that a sequence had before the call; its new token ``j`` stands at
 position ``starts + j``.  ``counts [B]`` (int32) limits the new tokens of a padded batch: token ``j`` of a sequence takes part
 when ``j < counts`` (default: all).  Places of one call must differ: two tokens written to one place leave either of them.
 
 bf16 / fp16 tensors on a GPU use the kernels of ``csrc/paged_cache.cu`` and ``csrc/paged_attention.cu`` (widths that are
 multiples of 16: heads up to 256, latents up to 512 with a rotary part up to 64); other types, widths and the CPU use
-:mod:`.reference`.  Nothing here is differentiable: inputs that need a gradient are refused.  No call waits for the GPU, and
-all of them can be captured into a CUDA graph.
+:mod:`.reference`.  Nothing here is differentiable: inputs that need a gradient are refused.  Calls on the kernels do not wait
+for the GPU and can be captured into a CUDA graph after a first call outside of it; the page table, starts and counts are read
+when the graph runs.  Rows, tables and lengths of layouts other than these are refused, queries, keys and values that are not
+aligned to 16 bytes are copied.
 """
 
 from __future__ import annotations
@@ -213,6 +216,8 @@ def paged_attention(
     _check_pages(op, k_pages, k_scale, q)
     _check_pages(op, v_pages, v_scale, q)
     _refuse(k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype, f"{op}: k_pages and v_pages differ")
+    _refuse(k_pages.stride(0) != v_pages.stride(0) or (k_scale is not None and k_scale.stride(0) != v_scale.stride(0)),
+            f"{op}: the pages of keys and values must lie equally far apart")
     _refuse(k_pages.shape[1] == 0 or q.shape[2] % k_pages.shape[1] != 0, f"{op}: the query heads must be a multiple of the cache's heads")
     _refuse(k_pages.shape[3] != q.shape[3], f"{op}: the cache has another dim than q")
     _refuse(k_scale is None and k_pages.dtype != q.dtype, f"{op}: the cache must have the query's type or be e4m3")

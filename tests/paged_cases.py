@@ -179,6 +179,7 @@ def refusals(device, dtype):
         "attention: pages transposed": att(k=su.k_pages.transpose(1, 2).contiguous().transpose(1, 2)),
         "attention: pages of 3 dims": att(k=su.k_pages[0], v=su.v_pages[0]),
         "attention: page of none": att(k=su.k_pages[:, :, :0], v=su.v_pages[:, :, :0]),
+        "attention: values further apart": att(v=torch.cat([su.v_pages, su.v_pages], 1)[:, :2]),
         "attention: values of other shape": att(v=su.v_pages[1:]),
         "attention: scales of a plain cache": att(ks=s8.k_scale, vs=s8.v_scale),
         "attention: no scales": att(k=s8.k_pages, v=s8.v_pages),

@@ -17,7 +17,7 @@ def test_attention(name, dtype, e4m3):
 
 
 @pytest.mark.parametrize("dtype,e4m3", TYPES, ids=str)
-@pytest.mark.parametrize("name", [n for n in pc.LATENT if n != "many-heads-long"])
+@pytest.mark.parametrize("name", ["one-token-cache", "ragged", "draft", "twenty-heads", "small-widths", "counts-missing"])
 def test_latent_attention(name, dtype, e4m3):
     pc.latent_case(pc.LATENT[name], dtype, e4m3, "cpu")
 
@@ -46,10 +46,9 @@ def test_hidden_values_that_are_not_finite(dtype, e4m3, window):
     pc.not_finite_case(dtype, e4m3, "cpu", window=window)
 
 
-@pytest.mark.parametrize("heads", [8, 64])
 @pytest.mark.parametrize("dtype,e4m3", TYPES, ids=str)
-def test_hidden_latents_that_are_not_finite(dtype, e4m3, heads):
-    pc.not_finite_case(dtype, e4m3, "cpu", latent=True, heads=heads)
+def test_hidden_latents_that_are_not_finite(dtype, e4m3):
+    pc.not_finite_case(dtype, e4m3, "cpu", latent=True)
 
 
 @pytest.mark.parametrize("dtype", [pc.F32, pc.BF], ids=str)

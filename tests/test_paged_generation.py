@@ -40,12 +40,12 @@ def test_same_tokens_as_the_dense_cache(name, length):
     torch.testing.assert_close(got_h, want_h, atol=2e-5, rtol=1e-4)
 
 
-@pytest.mark.parametrize("second", [1, 4, 20])
+@pytest.mark.parametrize("second", [1, 4, 140])
 @pytest.mark.parametrize("name", ["tiny-llama", "tiny-deepseek-v2"])
 def test_a_conversation_continues_in_the_cache(name, second):
     """A second prompt behind the first answer: the states are those of a plain forward over the whole text."""
     m = _model(name)
-    cache = PagedKVCache.for_model(m.config, 2, 80, page=16, dtype=torch.float32)
+    cache = PagedKVCache.for_model(m.config, 2, 200, page=16, dtype=torch.float32)
     first, _ = generate(m, _prompt(m, 2, 20), 6, do_sample=False, cache=cache)
     more = torch.cat([first[:, -1:], _prompt(m, 2, second, seed=5)], dim=1)
     answer, hidden = generate(m, more, 4, do_sample=False, cache=cache)

@@ -99,13 +99,88 @@ def _attention_inputs(starts, S=1, hq=16, hkv=4, d=128, e4m3=False, seed=0):
     return su, su.normal(su.B, S, hq, d)
 
 
+def _latent_inputs(starts, h, S=1, e4m3=False, seed=0):
+    su = pc.set_up(dict(starts=starts, S=S, page=64), pc.BF, e4m3, "cuda", values=False, d=576, seed=seed)
+    q, q_pe = su.normal(su.B, S, h, 512), su.normal(su.B, S, h, 64)
+    return lambda: ops.paged_latent_attention(q, q_pe, su.k_pages, su.table, su.starts, None, su.k_scale, 0.07)
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_same_bits_every_time(e4m3):
+    """Also with another call between, whose workspace may be the same memory, and without any wait."""
     su, q = _attention_inputs([5000, 17, 1234, 900], e4m3=e4m3)
-    args = (su.k_pages, su.v_pages, su.table, su.starts, None, su.k_scale, su.v_scale)
-    first = ops.paged_attention(q, *args)
-    for _ in range(5):
-        assert torch.equal(ops.paged_attention(q, *args).view(torch.int16), first.view(torch.int16))
+    other, oq = _attention_inputs([700, 2500, 9, 40, 41], e4m3=e4m3, seed=5)
+
+    def of(s, x):
+        return lambda: ops.paged_attention(x, s.k_pages, s.v_pages, s.table, s.starts, None, s.k_scale, s.v_scale)
+
+    calls = [of(su, q), of(other, oq)] + [_latent_inputs([3000, 17, 800], h, e4m3=e4m3, seed=h) for h in (16, 40, 128)]
+    first = []
+    for f in calls:
+        first.append(f())
+        torch.cuda.synchronize()
+    got = [(i, calls[i]()) for _ in range(6) for i in (0, 1, 2, 4, 3, 0, 4, 1)]
+    for i, x in got:
+        assert torch.equal(x.view(torch.int16), first[i].view(torch.int16)), i
+
+
+@pytest.mark.parametrize("h", [16, 128])
+def test_latent_attention_captured_and_on_two_streams(h):
+    calls = [_latent_inputs([2500, 3], h, seed=1), _latent_inputs([900, 1700, 64], h, seed=2)]
+    want = [f() for f in calls]
+    graphs, outs = [], []
+    for f in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(f())
+        graphs.append(graph)
+    for _ in range(3):
+        for x in outs:
+            x.zero_()
+        for graph in graphs:
+            graph.replay()
+        assert all(torch.equal(x, w) for x, w in zip(outs, want))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(calls[i]())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+    assert torch.ops.atb200.read_and_clear_error_flag(want[0]) == 0
+
+
+def test_a_captured_generation_step():
+    """Append and attention of a decoding step in one graph, replayed while the cache grows: lengths are read on the device."""
+    from arctictraining_b200.models import PagedKVCache
+
+    def normal(*shape):
+        return torch.randn(*shape, device="cuda").to(pc.BF)
+
+    torch.manual_seed(0)
+    caches = [PagedKVCache(1, 2, 128, 3, 200, page=32, device="cuda") for _ in range(2)]
+    q, k, v, pos = normal(3, 1, 8, 128), normal(3, 1, 2, 128), normal(3, 1, 2, 128), torch.zeros(3, 1, 64, device="cuda")
+    for c in caches:
+        c.reserve(200)
+        c.k_pages[0].fill_(float("nan"))
+        c.v_pages[0].fill_(float("nan"))
+
+    def step(c):
+        return c.attend(0, c.append(0, q, k, v, pos.cos(), pos.sin()))
+
+    step(caches[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(caches[0])
+    for i in range(150):
+        for x in (q, k, v):
+            x.normal_()
+        pos.fill_(0.1 * i)
+        graph.replay()
+        assert torch.equal(out, step(caches[1])), i
+        for c in caches:
+            c.advance(1)
 
 
 def test_two_captured_graphs_replayed_in_turn():
