@@ -19,6 +19,7 @@ aligned to 16 bytes are copied.
 
 from __future__ import annotations
 
+import os
 from typing import Optional
 from typing import Tuple
 
@@ -27,9 +28,14 @@ import torch
 from . import _ext
 from . import reference as ref
 from .functional import _count
-from .functional import _use_kernels
 
 _HALF = (torch.bfloat16, torch.float16)
+
+
+def _use_kernels(t: torch.Tensor) -> bool:
+    """As in :mod:`.functional`, without its questions to the driver once the library is loaded: a decoding step makes this
+    call in every layer."""
+    return t.is_cuda and ((_ext._loaded is True and "ATB200_DISABLE_KERNELS" not in os.environ) or _ext.available())
 
 
 def _refuse(cond: bool, what: str) -> None:
@@ -38,8 +44,11 @@ def _refuse(cond: bool, what: str) -> None:
 
 
 def _no_grad(op: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError(f"{op}: the generation cache is not differentiable; call it under torch.no_grad()")
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t.requires_grad:
+            raise ValueError(f"{op}: the generation cache is not differentiable; call it under torch.no_grad()")
 
 
 def _check_pages(op: str, pages: torch.Tensor, scale: Optional[torch.Tensor], x: torch.Tensor) -> None:
