@@ -523,7 +523,7 @@ static void launch_latent_rows(AttnArgs a, int64_t B, const at::Tensor& q) {
 // The accumulator is rescaled only when a row's maximum grew by more than 2^8.  All waits are bounded.
 // Measured: 128 heads, 89585 positions in 32 sequences (25 GFLOP, 112 MB) 59 us: the products take 24 of them (1070 cycles a
 // tile of 32 keys, as the instruction rates say), queries, first keys, results and the joining of a CTA's two or three pieces
-// the rest; 8-bit 75 us (softmax with two exponentials a score); one sequence of 60000 positions 45 us.
+// the rest; 8-bit 78 us (the softmax, and the pass for the queries' magnitudes); one sequence of 60000 positions 45 us.
 namespace tc {
 constexpr int kThreads = 288, kKeys = 32, kRing = 4, kRows = 128, kCols = 256;
 constexpr int kSub = kKeys * 128;                       // 64 columns of a stage, 128-byte swizzled rows
@@ -1022,15 +1022,25 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
                 const float mz = m == -INFINITY ? 0.f : m, vz = mv == -INFINITY ? 0.f : mv;
                 uint32_t pr[16];
                 float l0 = 0.f, l1 = 0.f;
+                // 8-bit: 2^(x + log2 scale - mv) = 2^(x - m) scale 2^(m - mv).  Every product is finite (mv is at least m + log2 of
+                // that key's scale - 8), and what 2^(x - m) loses below 2^-126 would need values above 2^100 to be seen.
+                const float g = E4M3 ? exp2f(mz - vz) : 1.f;
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float e0 = exp2f(x[i] - mz), e1 = exp2f(x[i + 1] - mz);
-                    l0 += e0;
-                    l1 += e1;
-                    if constexpr (E4M3)
-                        pr[i / 2] = pack2<P>(x[i] == -INFINITY ? 0.f : exp2f(x[i] + lv[i] - vz),
-                                             x[i + 1] == -INFINITY ? 0.f : exp2f(x[i + 1] + lv[i + 1] - vz));
-                    else pr[i / 2] = pack2<P>(e0, e1);
+                for (int i = 0; i < 32; i += 4) {
+                    float e[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) e[k] = exp2f(x[i + k] - mz);
+                    l0 += e[0] + e[2];
+                    l1 += e[1] + e[3];
+                    if constexpr (E4M3) {
+                        const float4 sc = *reinterpret_cast<const float4*>(s_scale + st * kKeys + i);
+                        e[0] = e[0] * sc.x * g;
+                        e[1] = e[1] * sc.y * g;
+                        e[2] = e[2] * sc.z * g;
+                        e[3] = e[3] * sc.w * g;
+                    }
+                    pr[i / 2] = pack2<P>(e[0], e[1]);
+                    pr[i / 2 + 1] = pack2<P>(e[2], e[3]);
                 }
                 l += l0 + l1;
                 ptx::tmem_st_32x32b_x16(my + kS + (T & 1) * kKeys, pr);
@@ -1228,6 +1238,7 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& q_pe, c
     at::Tensor out = at::empty({B, S, H, R}, q.options());
     if (out.numel() == 0) return out;
     if (pages.size(0) == 0 || table.size(1) == 0) return out.zero_();
+    gemm_error_flag(q.device());  // made by the first call of either form, so that a later one can be captured
     const at::Tensor qc = rows16(q), pc = rows16(q_pe);
     AttnArgs a;
     a.q = qc.data_ptr(); a.q2 = pc.data_ptr();
