@@ -510,7 +510,7 @@ static void launch_latent_rows(AttnArgs a, int64_t B, const at::Tensor& q) {
 }
 
 // ---- latent attention of many heads -------------------------------------------------------------------------------------
-// With 64 heads or more a token's query rows fill the 128 rows of the tensor core's accumulator, and 242 multiply-adds a cached
+// Many heads of a token (the form is taken from 33 on) fill the 128 rows of the tensor core's accumulator, and 242 flops a cached
 // byte (128 heads) make the matrix rate the bound.  One CTA takes the 128 rows of a token's heads and half of the 512 value
 // columns: weighted values 256, two score buffers of 32 keys, and 384 of the 576 query columns as left operand fill the 512
 // columns of tensor memory; the other 192 query columns and four stages of 32 keys lie in shared memory.  A left operand in
