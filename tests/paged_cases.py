@@ -60,20 +60,19 @@ def p_type(dtype, e4m3):
     return F32 if dtype == F32 else HF if e4m3 else dtype
 
 
-def attention_case(c, dtype, e4m3, device):
+def attention_case(c, dtype, e4m3, device, scale=None):
     su = set_up(c, dtype, e4m3, device)
     q = su.normal(su.B, su.S, c["hq"], su.D) * 2
-    scale = su.D**-0.5
+    scale = su.D**-0.5 if scale is None else scale
     got = ops.paged_attention(q, su.k_pages, su.v_pages, su.table, su.starts, su.counts, su.k_scale, su.v_scale, scale, c.get("window"))
     assert got.dtype == dtype and got.shape == q.shape
     want, tol = po.attention(su, q, scale, c.get("window"), p_type=p_type(dtype, e4m3))
     po.check_attention(got, want, tol, "attention")
 
 
-def latent_case(c, dtype, e4m3, device):
+def latent_case(c, dtype, e4m3, device, scale=192**-0.5):
     su = set_up(c, dtype, e4m3, device, values=False, d=c["R"] + c["rope"])
     q, q_pe = su.normal(su.B, su.S, c["h"], c["R"]), su.normal(su.B, su.S, c["h"], c["rope"])
-    scale = 192**-0.5
     got = ops.paged_latent_attention(q, q_pe, su.k_pages, su.table, su.starts, su.counts, su.k_scale, scale)
     assert got.dtype == dtype and got.shape == q.shape
     want, tol = po.attention(su, torch.cat((q, q_pe), -1), scale, latent=c["R"], p_type=p_type(dtype, e4m3))
@@ -257,3 +256,22 @@ def not_finite_case(dtype, e4m3, device, latent=False, window=None, heads=8):
     assert torch.equal(fine, torch.isfinite(got))
     po.check_close(torch.where(fine, got, 0.0), torch.where(fine, want, 0.0),
                    torch.where(fine, tol * 1.01 + want.abs() * po.step(dtype) * 1.02 + po.floor(dtype), 0.0), "not finite")
+
+
+def one_bad_query_case(dtype, e4m3, device, heads, latent):
+    """A query with a NaN gets NaN; all others get what they get without it, bit for bit."""
+    c = dict(starts=[300, 40], S=2, hq=heads, hkv=1 if latent else 2, page=16)
+    su = set_up(c, dtype, e4m3, device, values=not latent, d=576 if latent else 128)
+    q, q_pe = su.normal(2, 2, heads, 512 if latent else 128), su.normal(2, 2, heads, 64)
+
+    def call():
+        if latent:
+            return ops.paged_latent_attention(q, q_pe, su.k_pages, su.table, su.starts, None, su.k_scale, 0.1)
+        return ops.paged_attention(q, su.k_pages, su.v_pages, su.table, su.starts, None, su.k_scale, su.v_scale)
+
+    want = call()
+    q[0, 1, 3, 7] = float("nan")
+    got = call()
+    assert torch.isnan(got[0, 1, 3]).all()
+    got[0, 1, 3] = want[0, 1, 3]
+    assert torch.equal(got, want) and torch.isfinite(want).all()

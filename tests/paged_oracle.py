@@ -161,7 +161,7 @@ def attention(su, q, scale, window=None, latent=None, p_type=None):
                 qq, kk, vv = q[b, j, h * G : (h + 1) * G], k[pid, h, off], v[pid, h, off]
                 s = qq @ kk.T * scale
                 pr = torch.softmax(s, -1)
-                d = ((qq.abs() @ kk.abs().T) * scale * (D + 8) + s.abs() * 8).amax(-1, keepdim=True) * 2.0**-24 + 2.0**-21
+                d = ((qq.abs() @ kk.abs().T) * abs(scale) * (D + 8) + s.abs() * 8).amax(-1, keepdim=True) * 2.0**-24 + 2.0**-21
                 mass = pr @ vv.abs()
                 out[b, j, h * G : (h + 1) * G] = pr @ vv
                 small = 0.0

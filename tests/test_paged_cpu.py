@@ -51,6 +51,12 @@ def test_hidden_latents_that_are_not_finite(dtype, e4m3):
     pc.not_finite_case(dtype, e4m3, "cpu", latent=True)
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.0])
+def test_scales_of_any_sign(scale):
+    pc.attention_case(pc.ATTENTION["draft-window"], pc.BF, False, "cpu", scale)
+    pc.latent_case(pc.LATENT["draft"], pc.BF, True, "cpu", scale)
+
+
 @pytest.mark.parametrize("dtype", [pc.F32, pc.BF], ids=str)
 @pytest.mark.parametrize("name", list(pc.refusals("cpu", pc.F32)))
 def test_refusals(name, dtype):

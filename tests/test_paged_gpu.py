@@ -73,6 +73,30 @@ def test_hidden_latents_that_are_not_finite(dtype, e4m3, heads):
     pc.not_finite_case(dtype, e4m3, "cuda", latent=True, heads=heads)
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.0])
+@pytest.mark.parametrize("dtype,e4m3", TYPES, ids=str)
+def test_scales_of_any_sign(dtype, e4m3, scale):
+    pc.attention_case(pc.ATTENTION["draft-window"], dtype, e4m3, "cuda", scale)
+    pc.latent_case(pc.LATENT["draft"], dtype, e4m3, "cuda", scale)
+    pc.latent_case(pc.LATENT["sixty-four-heads-draft"], dtype, e4m3, "cuda", scale)
+
+
+@pytest.mark.parametrize("heads,latent", [(8, False), (8, True), (40, True)])
+@pytest.mark.parametrize("dtype,e4m3", TYPES, ids=str)
+def test_one_bad_query(dtype, e4m3, heads, latent):
+    pc.one_bad_query_case(dtype, e4m3, "cuda", heads, latent)
+
+
+def test_counts_beyond_the_call_and_below_none():
+    """A count is limited to the call's tokens and to none."""
+    su, q = _attention_inputs([50, 60, 70], S=3)
+    args = (q, su.k_pages, su.v_pages, su.table, su.starts)
+    want = ops.paged_attention(*args)
+    counts = torch.tensor([3, 9, -4], dtype=torch.int32, device="cuda")
+    got = ops.paged_attention(*args, counts)
+    assert torch.equal(got[:2], want[:2]) and torch.equal(got[2], torch.zeros_like(got[2]))
+
+
 @pytest.mark.parametrize("shape", [(0, 1, 4, 2), (2, 0, 4, 2), (2, 1, 0, 2)])
 def test_empty_calls(shape):
     B, S, hq, hkv = shape
