@@ -28,6 +28,17 @@ __device__ __forceinline__ void load8(const float* src, float (&f)[8]) {
     f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
 }
 
+// A rotation of the pairs (x, y), products and sums rounded one by one: contracted, a value next to a rounding border would be
+// stored as its neighbour, and an 8-bit row would hold other bytes than the reference writes for the same input.
+__device__ __forceinline__ void rotate8(float (&x)[8], float (&y)[8], const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float u = x[i], w = y[i];
+        x[i] = __fsub_rn(__fmul_rn(u, c[i]), __fmul_rn(w, s[i]));
+        y[i] = __fadd_rn(__fmul_rn(w, c[i]), __fmul_rn(u, s[i]));
+    }
+}
+
 struct AppendArgs {
     const void *q, *k, *v;
     int64_t q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h;  // strides in elements
@@ -86,14 +97,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
         Vec8<T>::unpack(next_lo, x);
         Vec8<T>::unpack(next_hi, y);
         load(r + groups, next_lo, next_hi);
-        if (mine && kind != 2) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float u = x[i], w = y[i];
-                x[i] = u * c[i] - w * s[i];
-                y[i] = w * c[i] + u * s[i];
-            }
-        }
+        if (mine && kind != 2) rotate8(x, y, c, s);
         float inv = 1.f, scale = 1.f;
         if (E4M3) {
             float m = 0.f;
@@ -181,12 +185,7 @@ __global__ void __launch_bounds__(256) latent_append_kernel(const LatentAppendAr
             float c[8], s[8];
             load8(cos + lane * 8, c);
             load8(sin + lane * 8, s);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const float u = p[t], w = r[t];
-                p[t] = u * c[t] - w * s[t];
-                r[t] = w * c[t] + u * s[t];
-            }
+            rotate8(p, r, c, s);
         }
         if (pid < 0) return;  // the whole warp
         ss = warp_sum(ss);
@@ -259,12 +258,7 @@ __global__ void __launch_bounds__(256) latent_append_kernel(const LatentAppendAr
             load8(sin + lane * 8, s);
             Vec8<T>::unpack(lo[x], p);
             Vec8<T>::unpack(hi[x], r);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const float y = p[t], z = r[t];
-                p[t] = y * c[t] - z * s[t];
-                r[t] = z * c[t] + y * s[t];
-            }
+            rotate8(p, r, c, s);
             T* dst = (T*)a.q_out + (tok * a.H + h) * a.rope;
             *reinterpret_cast<uint4*>(dst + lane * 8) = Vec8<T>::pack(p);
             *reinterpret_cast<uint4*>(dst + half + lane * 8) = Vec8<T>::pack(r);
