@@ -127,12 +127,17 @@ class Attention(nn.Module):
         return ops.attention(q, k, v, ctx.cu_seqlens, ctx.max_seqlen, True, ctx.attn_impl, window=self.window)
 
     def _forward_cached(self, x: torch.Tensor, ctx: ForwardContext, residual: Optional[torch.Tensor]) -> torch.Tensor:
-        """Generation step: the new tokens' keys and values are appended to the layer's cache and the queries attend to
+        """Generation step over a dense cache."""
+        B, S, _ = x.shape
+        o = self.attend_cached(*self.project_qkv(x, ctx), ctx)
+        return _project_with_residual(self.o_proj, o.reshape(B, S, self.hq * self.d), residual)
+
+    def attend_cached(self, q, k, v, ctx: ForwardContext) -> torch.Tensor:
+        """The new tokens' (rotated) keys and values are appended to the layer's cache and the queries attend to
         everything cached so far (causally among the new tokens when a whole prompt is processed at once)."""
         import torch.nn.functional as F
 
-        B, S, _ = x.shape
-        q, k, v = self.project_qkv(x, ctx)
+        S = q.shape[1]
         past = ctx.kv_cache[self.layer_idx]
         if past is not None:
             k = torch.cat([past[0], k], dim=1)
@@ -141,11 +146,11 @@ class Attention(nn.Module):
         Sk = k.shape[1]
         mask = None
         if S > 1:
-            qpos = torch.arange(Sk - S, Sk, device=x.device).view(S, 1)
-            mask = torch.arange(Sk, device=x.device).view(1, Sk) <= qpos
+            qpos = torch.arange(Sk - S, Sk, device=q.device).view(S, 1)
+            mask = torch.arange(Sk, device=q.device).view(1, Sk) <= qpos
         o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attn_mask=mask,
                                            enable_gqa=(self.hq != self.hkv))
-        return _project_with_residual(self.o_proj, o.transpose(1, 2).reshape(B, S, self.hq * self.d), residual)
+        return o.transpose(1, 2)
 
     def forward(self, x: torch.Tensor, ctx: ForwardContext, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         B, S, _ = x.shape

@@ -73,7 +73,12 @@ class SwiftKVAttention(Attention):
             return super().forward(x, ctx)
         B, S, _ = x.shape
         q = ops.rope(self.q_proj_swiftkv(x).view(B, S, self.hq, self.d), ctx.cos, ctx.sin)
-        o = self.core(q, k_shared, v_shared, ctx)
+        if ctx.kv_cache is None:
+            o = self.core(q, k_shared, v_shared, ctx)
+        elif isinstance(ctx.kv_cache, list):
+            o = self.attend_cached(q, k_shared, v_shared, ctx)
+        else:
+            raise NotImplementedError("layers that share another layer's keys and values generate with the dense cache only")
         return self.o_proj(o.reshape(B, S, self.hq * self.d))
 
 
