@@ -134,7 +134,8 @@ class Attention(nn.Module):
 
     def attend_cached(self, q, k, v, ctx: ForwardContext) -> torch.Tensor:
         """The new tokens' (rotated) keys and values are appended to the layer's cache and the queries attend to
-        everything cached so far (causally among the new tokens when a whole prompt is processed at once)."""
+        everything cached so far (causally among the new tokens when a whole prompt is processed at once), in sliding-window
+        layers to the last ``window`` positions of it."""
         import torch.nn.functional as F
 
         S = q.shape[1]
@@ -143,11 +144,16 @@ class Attention(nn.Module):
             k = torch.cat([past[0], k], dim=1)
             v = torch.cat([past[1], v], dim=1)
         ctx.kv_cache[self.layer_idx] = (k, v)
+        if self.window is not None:  # positions that no new token sees
+            k, v = k[:, -(self.window + S - 1) :], v[:, -(self.window + S - 1) :]
         Sk = k.shape[1]
         mask = None
         if S > 1:
             qpos = torch.arange(Sk - S, Sk, device=q.device).view(S, 1)
-            mask = torch.arange(Sk, device=q.device).view(1, Sk) <= qpos
+            kpos = torch.arange(Sk, device=q.device).view(1, Sk)
+            mask = kpos <= qpos
+            if self.window is not None:
+                mask = mask & (kpos > qpos - self.window)
         o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attn_mask=mask,
                                            enable_gqa=(self.hq != self.hkv))
         return o.transpose(1, 2)

@@ -1,11 +1,13 @@
 # SPDX-License-Identifier: Apache-2.0
-"""The two caches of ``generate`` where they can go wrong: layers that share keys and values."""
+"""The two caches of ``generate`` where they can go wrong: layers that share keys and values, sliding windows on the
+dense cache."""
 
 import sys
 from pathlib import Path
 
 import pytest
 import torch
+from test_paged_generation import _model
 from test_paged_generation import _prompt
 
 from arctictraining_b200.models import PagedKVCache
@@ -50,3 +52,18 @@ def test_layers_that_share_keys_and_values_refuse_the_paged_cache(name):
     m = _swiftkv_model(name)
     with pytest.raises(NotImplementedError):
         generate(m, _prompt(m, 2, 7), 6, do_sample=False, cache=PagedKVCache.for_model(m.config, 2, 20, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("length", [1, 4, 19])
+def test_sliding_window_layers_on_the_dense_cache(length):
+    m = _model("tiny-llama", sliding_window=6, use_sliding_window=True)
+    want, _ = generate(m, _prompt(m, 2, length), 12, do_sample=False,
+                       cache=PagedKVCache.for_model(m.config, 2, 40, page=4, dtype=torch.float32))
+    ids, hidden = generate(m, _prompt(m, 2, length), 12, do_sample=False)
+    _same_as_a_plain_forward(m, ids, hidden)
+    assert torch.equal(ids, want)
+
+
+def test_sliding_window_layers_that_share_keys_and_values():
+    m = _swiftkv_model("tiny-llama", sliding_window=6, use_sliding_window=True)
+    _same_as_a_plain_forward(m, *generate(m, _prompt(m, 2, 7), 6, do_sample=False))
