@@ -23,7 +23,10 @@ from .arch import ArchConfig
 class PagedKVCache:
     """``heads`` rows of ``dim`` elements per layer and position, for keys and for values; ``latent=True``: one joint row
     ``[latent | rotary key]`` instead.  ``num_pages`` pages are shared by ``batch`` sequences of up to ``max_length`` positions
-    (default: enough for all of them)."""
+    (default: enough for all of them).
+
+    A step is :meth:`reserve`, then :meth:`append` (or :meth:`append_latent`) and the attention of every layer, then
+    :meth:`advance`.  Positions that no page was reserved for are refused."""
 
     # New tokens per sequence that attend on the paged kernels; longer prompts read the cache back and use dense attention,
     # causal on an empty cache and with a mask behind earlier tokens (8 sequences of 4000 tokens, 32 heads on 8: 16 new tokens
@@ -56,6 +59,7 @@ class PagedKVCache:
         self.lengths: List[int] = [0] * batch  # the same on the host
         self._held: List[List[int]] = [[] for _ in range(batch)]
         self._free = list(range(self.num_pages - 1, -1, -1))
+        self._room = 0  # positions that every sequence has pages for, behind its cached ones
 
     @classmethod
     def for_model(cls, cfg: ArchConfig, batch: int, max_length: int, **kw) -> "PagedKVCache":
@@ -81,8 +85,14 @@ class PagedKVCache:
         if grew:
             self._upload()
 
+    def _check_room(self, tokens: int) -> None:
+        if tokens > self._room:
+            raise ValueError(f"PagedKVCache: {tokens} new positions, but some sequence has pages for {self._room} only; reserve them first")
+
     def advance(self, tokens: int) -> None:
         """The last ``tokens`` written positions of every sequence belong to it from now on (after all layers wrote them)."""
+        self._check_room(tokens)
+        self._room -= tokens
         self.lengths = [n + tokens for n in self.lengths]
         self.starts += tokens
 
@@ -98,6 +108,7 @@ class PagedKVCache:
         width = self.page_table.shape[1]
         rows = [held + [-1] * (width - len(held)) for held in self._held]
         self.page_table.copy_(torch.tensor(rows, dtype=torch.int32))
+        self._room = min(min(len(held) * self.page, self.max_length) - n for held, n in zip(self._held, self.lengths))
 
     def positions(self, tokens: int) -> torch.Tensor:
         """Position ids ``[batch, tokens]`` of the next tokens."""
@@ -110,10 +121,12 @@ class PagedKVCache:
     # -- one layer --------------------------------------------------------------------------------
     def append(self, layer: int, q, k, v, cos, sin) -> torch.Tensor:
         """Rotates the new tokens' queries and keys, stores keys and values, returns the queries."""
+        self._check_room(q.shape[1])
         return ops.paged_kv_append(q, k, v, cos, sin, self.k_pages[layer], self.v_pages[layer], self.page_table, self.starts, None,
                                    self.k_scale[layer], self.v_scale[layer])
 
     def append_latent(self, layer: int, q_pe, kv_a, norm_weight, eps: float, cos, sin) -> torch.Tensor:
+        self._check_room(q_pe.shape[1])
         return ops.paged_latent_append(q_pe, kv_a, norm_weight, eps, cos, sin, self.k_pages[layer], self.page_table, self.starts, None,
                                        self.k_scale[layer])
 

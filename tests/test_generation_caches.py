@@ -1,6 +1,6 @@
 # SPDX-License-Identifier: Apache-2.0
 """The two caches of ``generate`` where they can go wrong: layers that share keys and values, sliding windows on the
-dense cache."""
+dense cache, positions that nobody reserved."""
 
 import sys
 from pathlib import Path
@@ -67,3 +67,49 @@ def test_sliding_window_layers_on_the_dense_cache(length):
 def test_sliding_window_layers_that_share_keys_and_values():
     m = _swiftkv_model("tiny-llama", sliding_window=6, use_sliding_window=True)
     _same_as_a_plain_forward(m, *generate(m, _prompt(m, 2, 7), 6, do_sample=False))
+
+
+def _layer_inputs(c, S):
+    return [torch.zeros(c.batch, S, 2, 16)] * 3 + [torch.ones(c.batch, S, 8), torch.zeros(c.batch, S, 8)]
+
+
+def test_positions_that_nobody_reserved_are_refused():
+    c = PagedKVCache(1, 2, 16, batch=2, max_length=40, page=8, dtype=torch.float32)
+    latent = PagedKVCache(1, 1, 48, batch=2, max_length=40, page=8, latent=True, dtype=torch.float32)
+    with pytest.raises(ValueError):
+        c.append(0, *_layer_inputs(c, 1))
+    with pytest.raises(ValueError):
+        latent.append_latent(0, torch.zeros(2, 1, 2, 16), torch.zeros(2, 1, 48), torch.ones(32), 1e-6, torch.ones(2, 1, 8), torch.zeros(2, 1, 8))
+    with pytest.raises(ValueError):
+        c.advance(1)
+    assert c.lengths == [0, 0]
+    c.reserve(3)  # a page of eight each
+    c.append(0, *_layer_inputs(c, 8))
+    with pytest.raises(ValueError):
+        c.append(0, *_layer_inputs(c, 9))
+    with pytest.raises(ValueError):
+        c.advance(30)
+    c.advance(8)
+    assert c.lengths == [8, 8] and c.starts.tolist() == [8, 8]
+    with pytest.raises(ValueError):
+        c.append(0, *_layer_inputs(c, 1))
+    c.reserve(1)
+    c.append(0, *_layer_inputs(c, 1))
+    c.release(1)  # its next position has no page, as on a fresh cache
+    with pytest.raises(ValueError):
+        c.append(0, *_layer_inputs(c, 1))
+    c.reserve(1)
+    c.append(0, *_layer_inputs(c, 1))
+    c.advance(1)
+    assert c.lengths == [9, 1]
+
+
+def test_no_position_beyond_the_largest_length():
+    c = PagedKVCache(1, 2, 16, batch=2, max_length=21, page=8, dtype=torch.float32)  # three pages each hold 24
+    c.reserve(21)
+    with pytest.raises(ValueError):
+        c.append(0, *_layer_inputs(c, 22))
+    c.append(0, *_layer_inputs(c, 21))
+    c.advance(21)
+    with pytest.raises(ValueError):
+        c.advance(1)
