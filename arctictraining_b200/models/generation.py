@@ -17,6 +17,8 @@ from typing import Tuple
 import torch
 import torch.nn.functional as F
 
+from ..comm import errors
+from ..comm import get_rank
 from .kv_cache import PagedKVCache
 
 
@@ -36,7 +38,9 @@ def generate(
     token ``t + 1``).
 
     With a paged ``cache`` the prompt continues what the cache holds (``input_ids`` are the tokens behind it), and every token
-    that was fed to the model stays there: all but the last one returned, which starts the next call's prompt."""
+    that was fed to the model stays there: all but the last one returned, which starts the next call's prompt.  A kernel's
+    bounded wait that ran out meanwhile is raised at the end (once, so that the steps wait for nothing); what the cache holds is
+    then incomplete."""
     assert input_ids.dim() == 2, "generate: input_ids must be [batch, length]"
     B, S0 = input_ids.shape
     dev = input_ids.device
@@ -74,4 +78,6 @@ def generate(
         tokens = torch.cat([tokens, nxt], dim=1)
         pos0 += S
         step_ids = nxt
+    if cache is not None:
+        errors.raise_for_error_words(*errors.read_error_words(tokens), get_rank())
     return tokens, torch.cat(hidden_parts, dim=1)

@@ -1,6 +1,6 @@
 # SPDX-License-Identifier: Apache-2.0
 """The two caches of ``generate`` where they can go wrong: layers that share keys and values, sliding windows on the
-dense cache, positions that nobody reserved."""
+dense cache, positions that nobody reserved, and a device wait that ran out."""
 
 import sys
 from pathlib import Path
@@ -113,3 +113,24 @@ def test_no_position_beyond_the_largest_length():
     c.advance(21)
     with pytest.raises(ValueError):
         c.advance(1)
+
+
+@pytest.mark.parametrize("cached", [True, False])
+def test_a_device_wait_that_ran_out_is_raised_at_the_end(monkeypatch, cached):
+    """The error words of the device, here the host's stand-in for them, are read once per generation."""
+    from arctictraining_b200.comm import errors
+    from arctictraining_b200.exceptions import KernelWaitError
+
+    m = _model("tiny-llama")
+    reads = []
+    monkeypatch.setattr(errors, "read_error_words", lambda like: reads.append(like) or (0x3101, 0))
+    cache = PagedKVCache.for_model(m.config, 2, 20, dtype=torch.float32) if cached else None
+    if cached:
+        with pytest.raises(KernelWaitError):
+            generate(m, _prompt(m, 2, 4), 3, do_sample=False, cache=cache)
+        assert len(reads) == 1
+        monkeypatch.setattr(errors, "read_error_words", lambda like: (0, 0))
+        cache.release(0)
+        cache.release(1)
+    assert generate(m, _prompt(m, 2, 4), 3, do_sample=False, cache=cache)[0].shape == (2, 7)
+    assert len(reads) == int(cached)
