@@ -995,7 +995,9 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
                         v1 = fmaxf(v1, x[i + 1] + lv[i + 1]);
                     }
                 }
-                const float tm = fmaxf(t0, t1), tv = E4M3 ? fmaxf(v0, v1) : tm;
+                // the values' reference stays within 2^118 of the sum's: keys of scale 0 may hold the largest scores alone, and 2^(m - mv)
+                // below has to be finite (both references lag by up to 2^8)
+                const float tm = fmaxf(t0, t1), tv = E4M3 ? fmaxf(fmaxf(v0, v1), tm - 118.f) : tm;
                 if (tm > m + (m == -INFINITY ? 0.f : kGrow)) {
                     l *= m == -INFINITY ? 0.f : exp2f(m - tm);
                     m = tm;
@@ -1022,8 +1024,8 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
                 const float mz = m == -INFINITY ? 0.f : m, vz = mv == -INFINITY ? 0.f : mv;
                 uint32_t pr[16];
                 float l0 = 0.f, l1 = 0.f;
-                // 8-bit: 2^(x + log2 scale - mv) = 2^(x - m) scale 2^(m - mv).  Every product is finite (mv is at least m + log2 of
-                // that key's scale - 8), and what 2^(x - m) loses below 2^-126 would need values above 2^100 to be seen.
+                // 8-bit: 2^(x + log2 scale - mv) = 2^(x - m) scale 2^(m - mv).  Every product is finite: mv is at least m - 126 and
+                // x + log2 scale - 8.  What 2^(x - m) loses below 2^-126 would need values above 2^100 to be seen.
                 const float g = E4M3 ? exp2f(mz - vz) : 1.f;
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {

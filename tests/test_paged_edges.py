@@ -1,5 +1,5 @@
 # SPDX-License-Identifier: Apache-2.0
-"""Edges of the paged-cache operators: the bytes of an append."""
+"""Edges of the paged-cache operators: the bytes of an append, scales of zero."""
 
 import paged_cases as pc
 import pytest
@@ -7,6 +7,7 @@ import torch
 
 from arctictraining_b200 import ops
 
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 HALF = [(pc.BF, False), (pc.HF, False), (pc.BF, True), (pc.HF, True)]
 
 
@@ -41,3 +42,35 @@ def test_latent_append_rotates_like_the_reference(dtype):
         q = ops.paged_latent_append(*x, su.k_pages, su.table, su.starts)
         got.append((q.cpu(), su.k_pages[..., 512:].cpu().contiguous().view(torch.int16)))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("heads,latent", [(8, False), (16, True), (64, True), (128, True)])
+@pytest.mark.parametrize("log2_score,byte,scale", [(-127, -64.0, 2.0**-6), (-200, -1.0, 1.0), (-100, -128.0, 2.0**12), (-126, -256.0, 2.0**-20),
+                                                   (-1, -64.0, 2.0**-120)])
+def test_keys_with_a_scale_of_zero(device, heads, latent, log2_score, byte, scale):
+    """A row of zeros with a scale of zero (a position of a zero-filled cache) has score 0; the others are far below it.  Their
+    weight is 2^log2_score each; weights below 2^-126 may be lost, others are off by the usual roundings."""
+    D, n = (576 if latent else 64), 40
+    hkv = 1 if latent else 2
+    pages = torch.full((3, hkv, 16, D), byte, device=device).to(torch.float8_e4m3fn)
+    scales = torch.full((3, hkv, 16), scale, device=device)
+    pages.view(torch.uint8)[1, :, 5] = 0
+    scales[1, :, 5] = 0.0
+    table, starts = torch.tensor([[0, 1, 2]], dtype=torch.int32, device=device), torch.tensor([n - 1], dtype=torch.int32, device=device)
+    q = torch.ones(1, 1, heads, D, device=device, dtype=pc.BF)
+    by = log2_score * 0.6931471805599453 / (D * byte * scale)  # the scores are D byte scale
+    if latent:
+        got = ops.paged_latent_attention(q[..., :512], q[..., 512:], pages, table, starts, None, scales, by)
+    else:
+        got = ops.paged_attention(q, pages, pages, table, starts, None, scales, scales, by)
+    got = got.cpu().double()
+    assert torch.isfinite(got).all()
+    weight = 2.0**log2_score
+    want = (n - 1) * weight * byte * scale / (1 + (n - 1) * weight)
+    # the exponent |log2_score| is a product of two fp32 roundings and a sum of D equal products (D roundings at most): it is off by
+    # (D + 8) 2^-24 of itself at most, and the weight by 0.7 times that; its sums with a scale's logarithm and a maximum, all below
+    # 256, add four roundings of 2^-17; probabilities are rounded to fp16, the result to bf16.
+    slack = 0.7 * abs(log2_score) * (D + 8) * 2.0**-24 + 2.0**-15 + 2.0**-11 + 2.0**-8
+    lost = (n - 1) * 2.0**-126 * abs(byte) * scale if log2_score < -125 else 0.0
+    assert bool(((got - want).abs() <= abs(want) * slack + lost + 2.0**-126).all()), (got.min(), got.max(), want)
