@@ -537,6 +537,13 @@ constexpr uint32_t kS = 256, kQCol = 320;               // columns of tensor mem
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr float kGrow = 8.f;
 
+// What a role has issued must not outlive the CTA, also where another role gave up: waits for it (bounded), whatever the others do.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (!ptx::mbar_try_wait(bar, parity))
+        if (ptx::globaltimer_ns() - t0 > 100000000ull) return;
+}
+
 struct Piece {
     int b, item, r0, n, row0, rows, half, token;
     bool whole, first;
@@ -581,7 +588,7 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
     int* scratch = reinterpret_cast<int*>(smem + kBars + 32 * 8);  // no static memory: the tiles' alignment
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBars);
     uint64_t *k_full = bars, *k_empty = bars + kRing, *s_full = bars + 2 * kRing, *p_full = s_full + 2, *pv_done = p_full + 2,
-             *q_full = pv_done + 2, *q_sync = q_full + 1;
+             *q_full = pv_done + 2, *q_sync = q_full + 1, *drained = q_sync + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* s_scale = reinterpret_cast<float*>(smem + kScale);
@@ -612,6 +619,7 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
         }
         ptx::mbar_init(q_full, 128);
         ptx::mbar_init(q_sync, 128);
+        ptx::mbar_init(drained, 1);
         *abort_flag = 0;
         ptx::fence_barrier_init();
         ptx::fence_proxy_async_smem();
@@ -728,7 +736,9 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
                 }
             }
             copies_wait<0>();
-            if (ok) hand_over(T);
+            hand_over(T);
+            if (tid == 0)
+                for (int t = max(0, T - kRing); t < T; ++t) drain(&k_full[t % kRing], (t / kRing) & 1);
         } else {
             uint4 now[9], ahead[9];
             float scale_now = 0.f, scale_ahead = 0.f;
@@ -823,6 +833,8 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
                 if (ok) ok = issue_values(T - 1, p.n > 1, p.half);
             }
             if (!ok) atomicCAS(error_flag, 0, (0x32 << 8) | 1);
+            ptx::mma_commit(drained);
+            drain(drained, 0);
         }
     } else {
         // -------------------------------------------------------------------------------- softmax: a query row a thread
