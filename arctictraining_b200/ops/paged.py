@@ -30,6 +30,7 @@ from . import reference as ref
 from .functional import _count
 
 _HALF = (torch.bfloat16, torch.float16)
+_LARGEST = torch.finfo(torch.float32).max
 
 
 def _use_kernels(t: torch.Tensor) -> bool:
@@ -41,6 +42,10 @@ def _use_kernels(t: torch.Tensor) -> bool:
 def _refuse(cond: bool, what: str) -> None:
     if cond:
         raise ValueError(what)
+
+
+def _check_scale(op: str, scale: float) -> None:
+    _refuse(not abs(scale) <= _LARGEST, f"{op}: scale must be a finite 32-bit number")
 
 
 def _no_grad(op: str, *tensors: torch.Tensor) -> None:
@@ -218,6 +223,7 @@ def paged_attention(
         _refuse(window < 1, f"{op}: window must be positive")
     if scale is None:
         scale = q.shape[-1] ** -0.5
+    _check_scale(op, scale)
     if _use_kernels(q) and q.dtype in _HALF and q.dim() == 4 and q.shape[-1] % 16 == 0 and 0 < q.shape[-1] <= 256:
         _count()
         return _ext.ops().paged_attention(q, k_pages, v_pages, page_table, starts, counts, k_scale, v_scale, scale, window or 0)
@@ -251,6 +257,7 @@ def paged_latent_attention(
     op = "paged_latent_attention"
     _no_grad(op, q_latent, q_pe)
     _refuse(scale is None, f"{op}: scale must be given")
+    _check_scale(op, scale)
     if _use_kernels(q_latent) and q_latent.dtype in _HALF and q_latent.dim() == 4 and _latent_widths_ok(q_latent.shape[-1], q_pe.shape[-1]):
         _count()
         return _ext.ops().paged_latent_attention(q_latent, q_pe, pages, page_table, starts, counts, page_scale, scale)

@@ -1,5 +1,6 @@
 # SPDX-License-Identifier: Apache-2.0
-"""Edges of the paged-cache operators: the bytes of an append, scales of zero."""
+"""Edges of the paged-cache operators: the bytes of an append, scales of zero, scales of attention that
+are no numbers."""
 
 import paged_cases as pc
 import pytest
@@ -74,3 +75,14 @@ def test_keys_with_a_scale_of_zero(device, heads, latent, log2_score, byte, scal
     slack = 0.7 * abs(log2_score) * (D + 8) * 2.0**-24 + 2.0**-15 + 2.0**-11 + 2.0**-8
     lost = (n - 1) * 2.0**-126 * abs(byte) * scale if log2_score < -125 else 0.0
     assert bool(((got - want).abs() <= abs(want) * slack + lost + 2.0**-126).all()), (got.min(), got.max(), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 1e39])
+def test_a_scale_that_is_no_number_is_refused(device, scale):
+    dtype = pc.BF
+    su, lat = pc.set_up(pc.ATTENTION["draft"], dtype, False, device), pc.set_up(pc.LATENT["draft"], dtype, False, device, values=False, d=576)
+    with pytest.raises(ValueError):
+        ops.paged_attention(su.normal(3, 5, 8, 64), su.k_pages, su.v_pages, su.table, su.starts, scale=scale)
+    with pytest.raises(ValueError):
+        ops.paged_latent_attention(lat.normal(3, 3, 16, 512), lat.normal(3, 3, 16, 64), lat.k_pages, lat.table, lat.starts, scale=scale)
