@@ -221,6 +221,7 @@ def paged_attention(
     _no_grad(op, q)
     if window is not None:
         _refuse(window < 1, f"{op}: window must be positive")
+        window = min(window, 2**31 - 1)  # longer than any sequence
     if scale is None:
         scale = q.shape[-1] ** -0.5
     _check_scale(op, scale)

@@ -1,6 +1,6 @@
 # SPDX-License-Identifier: Apache-2.0
 """Edges of the paged-cache operators: the bytes of an append, scales of zero, scales of attention that
-are no numbers."""
+are no numbers, long windows."""
 
 import paged_cases as pc
 import pytest
@@ -86,3 +86,12 @@ def test_a_scale_that_is_no_number_is_refused(device, scale):
         ops.paged_attention(su.normal(3, 5, 8, 64), su.k_pages, su.v_pages, su.table, su.starts, scale=scale)
     with pytest.raises(ValueError):
         ops.paged_latent_attention(lat.normal(3, 3, 16, 512), lat.normal(3, 3, 16, 64), lat.k_pages, lat.table, lat.starts, scale=scale)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31, 10**15])
+def test_a_window_longer_than_any_sequence(device, window):
+    su = pc.set_up(pc.ATTENTION["draft"], pc.BF, False, device)
+    q = su.normal(3, 5, 8, 64)
+    args = (q, su.k_pages, su.v_pages, su.table, su.starts)
+    assert torch.equal(ops.paged_attention(*args, window=window), ops.paged_attention(*args))
