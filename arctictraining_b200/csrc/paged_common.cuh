@@ -96,13 +96,22 @@ __device__ __forceinline__ float e4m3_scale(float amax) { return __fdiv_rn(max_n
 
 inline bool is_e4m3(const at::Tensor& t) { return t.scalar_type() == at::kFloat8_e4m3fn; }
 
+// whether every slice along the first dimension is dense (a dimension of one element may have any stride)
+inline bool dense_inside(const at::Tensor& t) {
+    int64_t step = 1;
+    for (int64_t i = t.dim() - 1; i > 0; --i) {
+        if (t.size(i) != 1 && t.stride(i) != step) return false;
+        step *= t.size(i);
+    }
+    return true;
+}
+
 // a cache tensor: device, layout, type against the inputs' type, scales when its elements are e4m3
 inline void check_pages(const char* op, const at::Tensor& pages, const c10::optional<at::Tensor>& scale, const at::Tensor& x) {
     ATB_ARG(pages.dim() == 4, op, ": pages must be [pages, heads, page, dim]");
     ATB_ARG(pages.size(2) > 0, op, ": a page holds at least one position");
     ATB_ARG(pages.device() == x.device(), op, ": all tensors must be on one device");
-    ATB_ARG(pages.stride(3) == 1 && pages.stride(2) == pages.size(3) && pages.stride(1) == pages.size(2) * pages.size(3),
-            op, ": the heads, positions and elements of a page must be dense");
+    ATB_ARG(dense_inside(pages), op, ": the heads, positions and elements of a page must be dense");
     ATB_ARG((reinterpret_cast<uintptr_t>(pages.data_ptr()) & 15) == 0 && (pages.stride(0) * pages.element_size()) % 16 == 0,
             op, ": pages must be 16-byte aligned");
     if (is_e4m3(pages)) {
@@ -110,7 +119,7 @@ inline void check_pages(const char* op, const at::Tensor& pages, const c10::opti
         ATB_ARG(scale->scalar_type() == at::kFloat && scale->dim() == 3 && scale->size(0) == pages.size(0) &&
                     scale->size(1) == pages.size(1) && scale->size(2) == pages.size(2),
                 op, ": scales must be fp32 [pages, heads, page]");
-        ATB_ARG(scale->stride(2) == 1 && scale->stride(1) == scale->size(2), op, ": the scales of a page must be dense");
+        ATB_ARG(dense_inside(*scale), op, ": the scales of a page must be dense");
         ATB_ARG(scale->device() == x.device(), op, ": all tensors must be on one device");
     } else {
         ATB_ARG(!scale.has_value(), op, ": scales belong to an e4m3 cache");

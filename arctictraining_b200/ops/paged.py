@@ -56,16 +56,25 @@ def _no_grad(op: str, *tensors: torch.Tensor) -> None:
             raise ValueError(f"{op}: the generation cache is not differentiable; call it under torch.no_grad()")
 
 
+def _dense_inside(t: torch.Tensor) -> bool:
+    """Whether every slice along the first dimension is dense (a dimension of one element may have any stride)."""
+    step = 1
+    for size, stride in zip(t.shape[:0:-1], t.stride()[:0:-1]):
+        if size != 1 and stride != step:
+            return False
+        step *= size
+    return True
+
+
 def _check_pages(op: str, pages: torch.Tensor, scale: Optional[torch.Tensor], x: torch.Tensor) -> None:
     _refuse(pages.dim() != 4, f"{op}: pages must be [pages, heads, page, dim]")
     _refuse(pages.shape[2] < 1, f"{op}: a page holds at least one position")
     _refuse(pages.device != x.device, f"{op}: all tensors must be on one device")
-    _, _, n, d = pages.shape
-    _refuse(pages.stride()[1:] != (n * d, d, 1), f"{op}: the heads, positions and elements of a page must be dense")
+    _refuse(not _dense_inside(pages), f"{op}: the heads, positions and elements of a page must be dense")
     if pages.dtype == torch.float8_e4m3fn:
         _refuse(scale is None, f"{op}: an e4m3 cache needs its scales")
         _refuse(scale.dtype != torch.float32 or scale.shape != pages.shape[:3], f"{op}: scales must be fp32 [pages, heads, page]")
-        _refuse(scale.stride()[1:] != (n, 1), f"{op}: the scales of a page must be dense")
+        _refuse(not _dense_inside(scale), f"{op}: the scales of a page must be dense")
         _refuse(scale.device != x.device, f"{op}: all tensors must be on one device")
     else:
         _refuse(scale is not None, f"{op}: scales belong to an e4m3 cache")

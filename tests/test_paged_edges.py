@@ -1,6 +1,6 @@
 # SPDX-License-Identifier: Apache-2.0
 """Edges of the paged-cache operators: the bytes of an append, scales of zero, scales of attention that
-are no numbers, long windows."""
+are no numbers, long windows, heads or positions of one with any stride."""
 
 import paged_cases as pc
 import pytest
@@ -95,3 +95,26 @@ def test_a_window_longer_than_any_sequence(device, window):
     q = su.normal(3, 5, 8, 64)
     args = (q, su.k_pages, su.v_pages, su.table, su.starts)
     assert torch.equal(ops.paged_attention(*args, window=window), ops.paged_attention(*args))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_dimensions_of_one_may_have_any_stride(device, e4m3):
+    """One head, or pages of one position, as views of tensors whose dimensions have another order: the same rows."""
+    for c in (dict(starts=[20, 70], S=2, hq=4, hkv=1, d=64, page=16), dict(starts=[20, 7], S=2, hq=4, hkv=3, d=64, page=1)):
+        su = pc.set_up(c, pc.BF, e4m3, device)
+        q = su.normal(2, 2, 3 * su.Hkv, 64)
+        k, v = su.normal(2, 2, su.Hkv, 64), su.normal(2, 2, su.Hkv, 64)
+        cos, sin = su.angles(64)
+
+        def turned(t):
+            return None if t is None else t.transpose(1, 2).clone(memory_format=torch.contiguous_format).transpose(1, 2)
+
+        def calls(kp, vp, ks, vs):
+            a = ops.paged_kv_append(q, k, v, cos, sin, kp, vp, su.table, su.starts, None, ks, vs)
+            return [a, ops.paged_attention(q, kp, vp, su.table, su.starts, None, ks, vs),
+                    *ops.paged_kv_read(kp, vp, su.table, su.starts, 30, ks, vs)]
+
+        mine = [turned(t) for t in (su.k_pages, su.v_pages, su.k_scale, su.v_scale)]
+        for a, b in zip(calls(*mine), calls(su.k_pages, su.v_pages, su.k_scale, su.v_scale)):
+            assert torch.equal(a, b)
