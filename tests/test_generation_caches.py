@@ -134,3 +134,33 @@ def test_a_device_wait_that_ran_out_is_raised_at_the_end(monkeypatch, cached):
         cache.release(1)
     assert generate(m, _prompt(m, 2, 4), 3, do_sample=False, cache=cache)[0].shape == (2, 7)
     assert len(reads) == int(cached)
+
+
+def _gpu_model(name, **overrides):
+    sizes = dict(hidden_size=256, head_dim=64) if name == "tiny-llama" else dict(kv_lora_rank=64, qk_rope_head_dim=32, qk_nope_head_dim=32,
+                                                                                 v_head_dim=32, head_dim=32)
+    return _model(name, torch.bfloat16, "cuda", **sizes, **overrides)
+
+
+def _off(m, text, hidden, first=0):
+    with torch.no_grad():
+        full = m(input_ids=text[:, :-1], hidden_only=True).hidden_states[:, first:]
+    return float((hidden.float() - full.float()).norm() / full.float().norm())
+
+
+# Two or three layers of about ten bf16 roundings of 2^-9 each add up to 3 * 10 * 2^-9 = 6 % at most; an 8-bit row's elements are off by
+# 2^-4 at most, and what attention makes of them by no more in models with weights of 0.02.
+@pytest.mark.gpu
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("second", [1, 4, 140])
+@pytest.mark.parametrize("name,window", [("tiny-llama", None), ("tiny-llama", 6), ("tiny-deepseek-v2", None)])
+def test_a_conversation_on_the_gpu(name, window, second, e4m3):
+    """A prompt, its answer, a second prompt of one, few and many tokens, and a second answer, in one cache."""
+    m = _gpu_model(name, **(dict(sliding_window=window, use_sliding_window=True) if window else {}))
+    limit = 0.06 + (2.0**-4 if e4m3 else 0.0)
+    cache = PagedKVCache.for_model(m.config, 2, 200, page=16, e4m3=e4m3, dtype=torch.bfloat16, device="cuda")
+    first, hidden = generate(m, _prompt(m, 2, 20), 6, do_sample=False, cache=cache)
+    assert _off(m, first, hidden) < limit
+    more = torch.cat([first[:, -1:], _prompt(m, 2, second, seed=5)], dim=1)
+    answer, hidden = generate(m, more, 4, do_sample=False, cache=cache)
+    assert _off(m, torch.cat([first[:, :-1], answer], dim=1), hidden, first.shape[1] - 1) < limit

@@ -1,8 +1,10 @@
 # SPDX-License-Identifier: Apache-2.0
 """Edges of the paged-cache operators: the bytes of an append, scales of zero, scales of attention that
-are no numbers, long windows, heads or positions of one with any stride."""
+are no numbers, long windows, heads or positions of one with any stride, more
+sequences than a block has threads."""
 
 import paged_cases as pc
+import paged_oracle as po
 import pytest
 import torch
 
@@ -118,3 +120,20 @@ def test_dimensions_of_one_may_have_any_stride(device, e4m3):
         mine = [turned(t) for t in (su.k_pages, su.v_pages, su.k_scale, su.v_scale)]
         for a, b in zip(calls(*mine), calls(su.k_pages, su.v_pages, su.k_scale, su.v_scale)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [None, 16, 40])
+@pytest.mark.parametrize("batch", [129, 384, 1000])
+def test_more_sequences_than_a_block_has_threads(batch, heads):
+    """The division of the work gives a thread several sequences then, some of them with one position only."""
+    lengths = [(i * 37) % 90 for i in range(batch)]
+    su = pc.set_up(dict(starts=lengths, S=1, page=16, hkv=1 if heads else 2), pc.BF, False, "cuda", values=heads is None, d=576 if heads else 64)
+    q, q_pe = su.normal(batch, 1, heads or 8, 512 if heads else 64), su.normal(batch, 1, heads or 8, 64)
+    if heads:
+        got = ops.paged_latent_attention(q, q_pe, su.k_pages, su.table, su.starts, None, None, 0.07)
+        want, tol = po.attention(su, torch.cat((q, q_pe), -1), 0.07, latent=512, p_type=pc.BF)
+    else:
+        got = ops.paged_attention(q, su.k_pages, su.v_pages, su.table, su.starts)
+        want, tol = po.attention(su, q, 64**-0.5, p_type=pc.BF)
+    po.check_attention(got, want, tol, "many sequences")
