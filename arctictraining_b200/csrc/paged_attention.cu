@@ -16,10 +16,13 @@ namespace paged {
 // so that probabilities stay within (0, 1] whatever the scales are.
 // Probabilities are rounded to the 16-bit type of the instruction (fp16 for e4m3 values): the same size of error as the
 // final rounding of the result.  Scores, maxima, sums and weighted values are fp32.
-// Measured: four 8-bit caches of up to 131000 positions (807 MB) 136 us, 92 % of a plain copy's rate; 64 sequences of 17 to 6100
-// positions (402 MB) 73 us, 85 %; one sequence of 777 positions 10 us (two launches and four dependent loads: lengths, page,
-// keys, pieces).  Drafts of five tokens in fp16 layers of 64-wide heads with a window of 4096 (156 MB) 43 us, 56 %: their
-// masked first and last tiles and two row tiles a warp.
+// Measured: four 8-bit caches of up to 131000 positions (807 MB) 138 us, 91 % of a plain copy's rate, in a short replay at 1965 MHz;
+// 162 us, 77 %, after a second of such calls, when the power limit lowers the clocks.  64 sequences of 17 to 6100 positions (402 MB)
+// 73 us, 85 %, and over 8-bit rows (208 MB) 54 us, 59 %; 256-wide heads, 24 sequences of 4000 positions (787 MB) 136 us, 89 %; one
+// sequence of 777 positions 10.6 us (two launches and four dependent loads: lengths, page, keys, pieces).  Drafts of five tokens in
+// fp16 layers of 64-wide heads with a window of 4096 (156 MB) 44 us, 55 %: eight warps an SM, stalled on fixed latencies.  Many new
+// tokens are far from the floor (8 sequences of 4000 positions, 32 heads on 8: 64 tokens 180 us of 22, 128 tokens 365 us of 41):
+// every tile of 64 query rows reads all keys of its cache head, those hidden from all its rows too.
 constexpr int kStages = 3;
 
 template <bool E4M3, int DP>

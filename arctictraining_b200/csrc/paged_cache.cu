@@ -57,8 +57,8 @@ struct AppendArgs {
 // sin of a lane are loaded once and serve all heads of the token.  The next row is on its way while one is worked on, and the
 // place in the cache is looked up behind the first loads.  Few tokens get a wide CTA (all rows at once: latency counts),
 // many get narrow ones, 16 to an SM, whose fixed chain of loads (lengths, page, cos / sin) overlaps.
-// Measured: one token of 32 + 16 heads 2.2 us (launch); 12 prompts of up to 1511 tokens, 28 + 8 heads, into an 8-bit cache (301
-// MB) 51 us, 91 % of a plain copy's rate.
+// Measured: one token of 32 + 16 heads 2.6 us (launch); 12 prompts of up to 1511 tokens, 28 + 8 heads, into an 8-bit cache (301
+// MB) 52 us, 90 % of a plain copy's rate, and as they are (311 MB) 52 us, 93 %.
 template <typename T, bool E4M3, int LPR>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     const int64_t tok = blockIdx.x;
@@ -151,8 +151,9 @@ struct LatentAppendArgs {
 };
 
 // One CTA per new token: warp 0 normalises, rotates and writes the latent row (16 latent elements a lane, the rotary part on
-// its first lanes), the others (enough for two rounds over all heads) rotate the queries.  Measured: 96 tokens 2.8 us; 8 prompts
-// of up to 2048 tokens (97 MB) 21 us, 71 % of a plain copy's rate (fixed chain of loads per token).
+// its first lanes), the others (enough for two rounds over all heads) rotate the queries.  Measured: 96 tokens 3.0 us; 8 prompts
+// of up to 2048 tokens (97 MB) 21 us, 71 % of a plain copy's rate, into 8-bit rows (90 MB) 22 us, 63 %: a token's chain of lengths,
+// row or page, weight and write, with nothing of the next token on its way.
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(256) latent_append_kernel(const LatentAppendArgs a) {
     const int64_t tok = blockIdx.x;
@@ -279,7 +280,7 @@ struct ReadArgs {
 
 // One CTA per kReadRows rows (position, head) of one sequence's keys or values.  The places of the rows are looked up once, into
 // shared memory; then every thread moves 16-byte pieces of the result, four on their way at a time.  Measured: 16 sequences of
-// up to 16000 8-bit latent rows (392 MB) 66.5 us, 91 % of a plain copy's rate.
+// up to 16000 8-bit latent rows (392 MB) 67 us, 91 % of a plain copy's rate, and plain ones (488 MB) 80 us, 94 %.
 constexpr int kReadRows = 64, kReadDim = 2048;  // 64 rows of at most 256 chunks
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {

@@ -17,9 +17,9 @@ namespace paged {
 // steps of 16 are divided over four groups of warps (whose slice of the queries stays in registers) and the keys over two, so
 // every key byte is read from shared memory once; the four partial sums meet in shared memory, where the softmax is taken by
 // all threads.  Weighted values: every warp reads its own 64 columns of the same tile.  Precision is that of the grouped form.
-// Measured with 16 heads: one sequence of 4003 positions 15 us; 89585 positions in 32 sequences (106 MB) 34 us, 48 % of a plain
+// Measured with 16 heads: one sequence of 4003 positions 15 us; 89585 positions in 32 sequences (104 MB) 34 us, 47 % of a plain
 // copy's rate (a tile of 64 keys takes 2 us, 1.75 of them its 74 KB; ten tiles a CTA do not hide the 7 us of an item's begin and
-// end and the joining); 32 heads 46 us.
+// end and the joining), 8-bit rows (53 MB) 33 us, 25 %; 32 heads 47 and 49 us.
 constexpr int kLatent = 512, kRotary = 64, kJoint = kLatent + kRotary;
 
 template <bool E4M3, int MT>
@@ -521,9 +521,10 @@ static void launch_latent_rows(AttnArgs a, int64_t B, const at::Tensor& q) {
 // (8-bit ones are turned into fp16 on the way).  Warp 8 issues the products; scores of the next tile run ahead of the values
 // of this one.  All keys that a row tile sees are the same for its rows (one token), so hidden keys are never fetched.
 // The accumulator is rescaled only when a row's maximum grew by more than 2^8.  All waits are bounded.
-// Measured: 128 heads, 89585 positions in 32 sequences (25 GFLOP, 112 MB) 59 us: the products take 24 of them (1070 cycles a
+// Measured: 128 heads, 89585 positions in 32 sequences (25 GFLOP, 112 MB) 60 us: the products take 24 of them (1070 cycles a
 // tile of 32 keys, as the instruction rates say), queries, first keys, results and the joining of a CTA's two or three pieces
-// the rest; 8-bit 78 us (the softmax, and the pass for the queries' magnitudes); one sequence of 60000 positions 45 us.
+// the rest, one after the other; 8-bit 79 us (the softmax, and the pass for the queries' magnitudes); one sequence of 60000 positions
+// 46 us; 4 sequences of 4000 positions with 64 new tokens 384 us of 172.
 namespace tc {
 constexpr int kThreads = 288, kKeys = 32, kRing = 4, kRows = 128, kCols = 256;
 constexpr int kSub = kKeys * 128;                       // 64 columns of a stage, 128-byte swizzled rows
@@ -788,8 +789,8 @@ latent_tc_kernel(const __grid_constant__ CUtensorMap tmap, int page_rows, const 
         if (!ok && lane == 0) atomicCAS(error_flag, 0, (0x31 << 8) | 1);
     } else if (warp == 8) {
         // -------------------------------------------------------------------------------- products
-        // The thread is chosen by elect.sync: the compiler then knows that one thread issues, and a product of 32 columns takes
-        // its 16 cycles (45 to 80 behind a test of the lane, which moves every operand to uniform registers one by one).
+        // The thread is chosen by elect.sync: a product of 32 columns was then measured at 16 cycles, and at 45 behind a test of
+        // the lane.
         if (ptx::elect_one()) {
             constexpr uint32_t fmt = std::is_same<P, bf16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t kind = ~((1u << 7) | (1u << 10));
@@ -1222,7 +1223,8 @@ static void launch_latent_tc(AttnArgs a, int64_t B, const at::Tensor& q) {
 template <typename T, bool E4M3>
 static void launch_latent(const AttnArgs& a, int64_t B, const at::Tensor& q) {
     // The tensor-core form from 33 heads on, where the other needs a second tile of 32 rows a token and with it the keys a
-    // second time (89585 positions: 32 heads 46 us in one tile; 48 heads 78 us in two and 55 us here, 64 heads 80 and 56 us).  Several tokens of few heads stay with the other: here each token has tiles of its own.
+    // second time (89585 positions: 32 heads 47 us in one tile; 48 heads 78 us in two and 55 us here, 64 heads 80 and 56 us).
+    // Several tokens of few heads stay with the other: here each token has tiles of its own.
     if (a.Hq > 32 && a.D1 == kLatent && a.D == kJoint) return launch_latent_tc<T, E4M3>(a, B, q);
     if (a.S * a.Hq <= 16) launch_latent_rows<T, E4M3, 1>(a, B, q);
     else launch_latent_rows<T, E4M3, 2>(a, B, q);

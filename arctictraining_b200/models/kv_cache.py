@@ -29,9 +29,11 @@ class PagedKVCache:
     :meth:`advance`.  Positions that no page was reserved for are refused."""
 
     # New tokens per sequence that attend on the paged kernels; longer prompts read the cache back and use dense attention,
-    # causal on an empty cache and with a mask behind earlier tokens (8 sequences of 4000 tokens, 32 heads on 8: 16 new tokens
-    # 60 us on the pages and 235 us dense, 128 tokens 336 and 434 us; latent, 4 x 4000 tokens, 128 heads: 64 tokens 0.43 and
-    # 4.4 ms).
+    # causal on an empty cache and with a mask behind earlier tokens.  Measured both ways for 1 to 64 sequences of 0 to 32000 cached
+    # tokens, 8 to 128 new ones, three head layouts, windows, 8-bit and latent rows.  Behind cached tokens the pages are ahead up to
+    # 128 new ones: 8 x 4000, 32 heads on 8, 16 new tokens 60 us and 236 dense, 128 tokens 338 and 436; 32 x 2000 683 and 781; at the
+    # least 64 x 200, 329 and 328; with a window of 512, 8 x 4000, 100 and 459; a latent layer of 128 heads, 4 x 4000, 64 tokens, 0.62
+    # and 4.7 ms.  On an empty cache 64 sequences of 16 tokens take 21 and 46 us, of 32 tokens 36 and 45, of 64 tokens 68 and 49.
     first_tokens, more_tokens = 16, 128
 
     def __init__(self, layers: int, heads: int, dim: int, batch: int, max_length: int, *, page: int = 64, e4m3: bool = False,

@@ -2,7 +2,7 @@
 """Operators of the paged generation cache.
 
 A cache is ``pages [P, heads, page, dim]``: page ``p`` holds ``page`` consecutive positions of one sequence.  Its elements
-have the model's type, or are e4m3 with one fp32 scale per position and head (``[P, heads, page]``).  ``page_table [B, W]``
+have the model's type, or are e4m3 with one fp32 scale of 0 or more per position and head (``[P, heads, page]``).  ``page_table [B, W]``
 (int32) names the pages of every sequence in order; an id outside ``[0, P)`` stands for no page: writes to it are dropped and
 reads skip it.  The heads, positions and elements of a page are dense; pages may lie further apart (slices of a larger tensor),
 keys and values equally far.  ``starts [B]`` (int32) are the tokens that a sequence had before the call; its new token ``j`` stands at
@@ -13,8 +13,10 @@ bf16 / fp16 tensors on a GPU use the kernels of ``csrc/paged_cache.cu`` and ``cs
 multiples of 16: heads up to 256, latents up to 512 with a rotary part up to 64); other types, widths and the CPU use
 :mod:`.reference`.  Nothing here is differentiable: inputs that need a gradient are refused.  Calls on the kernels do not wait
 for the GPU and can be captured into a CUDA graph after a first call outside of it; the page table, starts and counts are read
-when the graph runs.  Rows, tables and lengths of layouts other than these are refused, queries, keys and values that are not
-aligned to 16 bytes are copied.
+when the graph runs.  Rows, tables and lengths of layouts other than these, and on the kernels pages that do not start on 16 bytes,
+are refused; queries, keys and values that are not aligned to 16 bytes are copied.  Latent attention of many heads waits inside its
+kernel for a bounded time only: a wait that ran out leaves a code in the device's error word (:mod:`..comm.errors`), which the
+training engine and ``models.generation.generate`` read.
 """
 
 from __future__ import annotations
